@@ -1,0 +1,439 @@
+"""Workloads of the operators that run beside the 4-bit projections of a decoder: rotary positions, the 8-bit
+key/value cache (append, read back), attention over that cache, and low-rank adapters (forward, gradients).
+
+`run` computes an operator in elementary torch operations, or, where `own` is true, through popxl_addons."""
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+BLOCK = 64  # tokens of one block of the cache, the unit that has a scale of its own
+BASE = 10000.0
+
+
+def _framework():
+    path = os.path.join(os.getcwd(), "popxl-addons_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from popxl_addons.ops import kv_cache_gq, low_rank_adapters, rotary_pos_embed
+
+    return rotary_pos_embed, kv_cache_gq, low_rank_adapters
+
+
+# ------------------------------------------------------------------------------------------------- cases
+
+
+def listed():
+    return [
+        # one decode step of a small batch on the 6B layer (16 heads of 256, the first 64 of them rotated): latency
+        dict(name="rotary decode", op="rotary", tokens=4, heads=32, other=16, head_dim=256, rotary_dim=64, layout="interleaved",
+             scaling="", positions=2048, inverse=False),
+        # gradient of a long prompt's queries and keys, grouped heads, context stretched
+        dict(name="rotary long back", op="rotary", tokens=16381, heads=40, other=8, head_dim=128, rotary_dim=128, layout="half",
+             scaling="yarn", positions=131072, inverse=True),
+        # a decode step of 48 requests: one token each, most of them into a block that has tokens
+        dict(name="append decode", op="append", batch=48, new=1, context=4000, kv_heads=16, head_dim=256, rotary_dim=64,
+             layout="interleaved"),
+        # three prompts written at once
+        dict(name="append prompts", op="append", batch=3, new=5461, context=6000, kv_heads=8, head_dim=128, rotary_dim=128,
+             layout="half"),
+        # one request with a short history: latency
+        dict(name="attend one", op="attend", batch=1, new=1, context=777, q_heads=16, kv_heads=16, head_dim=256),
+        # decode of 64 requests of very different lengths, grouped heads
+        dict(name="attend many", op="attend", batch=64, new=1, context=32768, q_heads=32, kv_heads=8, head_dim=128),
+        # a prompt's chunk of the 6B layer behind its own earlier chunks
+        dict(name="attend chunk", op="attend", batch=2, new=2048, context=8000, q_heads=16, kv_heads=16, head_dim=256),
+        # decode batch, every request with an adapter of its own or none
+        dict(name="adapt decode", op="adapt", rows=8, k=4096, n=4096, rank=16, adapters=12, none=True, runs=False, activation=""),
+        # a larger decode batch on the feed-forward's first projection, activation behind the sum
+        dict(name="adapt batch", op="adapt", rows=150, k=4096, n=16384, rank=64, adapters=40, none=True, runs=False,
+             activation="gelu_tanh"),
+        # prompts of several requests, each with its adapter
+        dict(name="adapt prompts", op="adapt", rows=6001, k=4096, n=12288, rank=32, adapters=5, none=False, runs=True, activation=""),
+        # a small training batch of mixed tasks
+        dict(name="adapt back small", op="adapt_back", rows=511, k=4096, n=4096, rank=8, adapters=3, none=True, runs=True),
+        # training of one adapter on the feed-forward's first projection
+        dict(name="adapt back", op="adapt_back", rows=8192, k=4096, n=16384, rank=64, adapters=1, none=False, runs=True),
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(["rotary", "append", "attend", "attend", "adapt", "adapt", "adapt_back"])
+    head_dim = rng.choice([64, 80, 96, 128, 256])
+    layout = rng.choice(["interleaved", "half"])
+    rotary_dim = rng.choice([32, 64, head_dim]) if head_dim > 64 else rng.choice([32, 64])
+    if op == "rotary":
+        return dict(op=op, tokens=_log(rng, 1, 8000), heads=rng.randint(1, 40), other=rng.choice([0, 1, 8]), head_dim=head_dim,
+                    rotary_dim=rotary_dim, layout=layout, scaling=rng.choice(["", "linear", "ntk", "yarn"]),
+                    positions=_log(rng, 64, 1 << 20), inverse=rng.random() < 0.5)
+    if op == "append":
+        new = rng.choice([1, _log(rng, 2, 3000)])
+        return dict(op=op, batch=_log(rng, 1, 64) if new == 1 else rng.randint(1, 4), new=new, context=new + _log(rng, 1, 4000),
+                    kv_heads=rng.choice([1, 2, 5, 8, 16]), head_dim=head_dim, rotary_dim=rotary_dim, layout=layout)
+    if op == "attend":
+        kv_heads = rng.choice([1, 2, 4, 8, 16])
+        kind = rng.choice(["one", "few", "chunk"])
+        if kind == "one":
+            return dict(op=op, batch=_log(rng, 1, 32), new=1, context=_log(rng, 1, 12000), q_heads=kv_heads * rng.choice([1, 1, 4, 7, 8]),
+                        kv_heads=kv_heads, head_dim=head_dim)
+        if kind == "few":
+            new = rng.randint(2, 9)
+            return dict(op=op, batch=_log(rng, 1, 32), new=new, context=new + _log(rng, 1, 8000), q_heads=kv_heads * rng.choice([1, 4, 8]),
+                        kv_heads=kv_heads, head_dim=head_dim)
+        new = _log(rng, 17, 1000)
+        return dict(op=op, batch=rng.randint(1, 2), new=new, context=new + _log(rng, 1, 4000), q_heads=min(32, kv_heads * rng.choice([1, 4])),
+                    kv_heads=kv_heads, head_dim=head_dim)
+    k, n = rng.choice([(4096, 4096), (4096, 16384), (16384, 4096), (1024, 4096), (2048, 520), (1000, 1016)])
+    rank = rng.choice([4, 8, 13, 16, 32, 64])
+    if op == "adapt":
+        rows = _log(rng, 1, 4000)
+        return dict(op=op, rows=rows, k=k, n=n, rank=rank, adapters=rng.choice([1, 3, 16, 50]), none=rng.random() < 0.5, runs=rows > 256,
+                    activation=rng.choice(["", "", "relu", "gelu_tanh"]))
+    return dict(op=op, rows=_log(rng, 16, 4000), k=k, n=n, rank=rank, adapters=rng.choice([1, 2, 7]), none=rng.random() < 0.5, runs=True)
+
+
+# ------------------------------------------------------------------------------------------------- inputs
+
+
+def _lengths(case, order):
+    """(lengths, new tokens) of every sequence: evenly spread up to the largest, in an order that the seed gives."""
+    b, new, context = case["batch"], case["new"], case["context"]
+    pairs = []
+    for i in range(b):
+        fresh = new if new == 1 else max(1, new * (i + b) // (2 * b - 1) if b > 1 else new)
+        pairs.append((max(fresh, context * (i + 1) // b), fresh))
+    order.shuffle(pairs)
+    return [p[0] for p in pairs], [p[1] for p in pairs]
+
+
+def _normal(gen, *shape, std=1.0, dtype=torch.float16):
+    return (torch.randn(*shape, generator=gen, device="cuda") * std).to(dtype)
+
+
+def _frequencies(case):
+    """Radians a position, in 64 bits, and the factor of the rotated values."""
+    r, scaling = case["rotary_dim"], case.get("scaling", "")
+    i = torch.arange(0, r, 2, dtype=torch.float64) / r
+    if scaling == "ntk":
+        return (BASE * 4.0 ** (r / (r - 2))) ** -i, 1.0
+    w = BASE ** -i
+    if scaling == "linear":
+        return w / 4.0, 1.0
+    if scaling == "yarn":
+        keep = ((4096 * w / (2 * math.pi) - 1.0) / (32.0 - 1.0)).clamp(0, 1)
+        return w / 8.0 * (1 - keep) + w * keep, 0.1 * math.log(8.0) + 1.0
+    return w, 1.0
+
+
+_SCALING = {"": None, "linear": dict(kind="linear", factor=4.0), "ntk": dict(kind="ntk", factor=4.0),
+            "yarn": dict(kind="yarn", factor=8.0, original_length=4096)}
+
+
+def _paged(case, gen, order, state):
+    """The cache as it lies in memory, its blocks in no order, with the histories of all sequences in it."""
+    lengths, fresh = _lengths(case, order)
+    h, d = case["kv_heads"], case["head_dim"]
+    need = [-(-n // BLOCK) for n in lengths]
+    total = sum(need) + 3
+    ids = list(range(total))
+    order.shuffle(ids)
+    table = torch.zeros(len(lengths), max(need), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = torch.tensor(ids[at:at + n], dtype=torch.int32)
+        at += n
+    offsets = torch.tensor([0] + fresh, dtype=torch.int32).cumsum(0).to(torch.int32)
+    # (codes of normal values whose largest takes the whole range; drawn in bytes, since long caches are large)
+    def codes(*shape):
+        c = torch.empty(shape, dtype=torch.uint8, device="cuda")
+        for part in c.split(max(1, (1 << 26) // (h * d * BLOCK))):
+            part.copy_((torch.randn(part.shape, generator=gen, device="cuda") * 36 + 128).round().clamp(1, 255))
+        return c
+
+    state.update(case=case, lengths=lengths, fresh=fresh, offsets=offsets.cuda(), seq_lens=torch.tensor(lengths, dtype=torch.int32).cuda(),
+                 table=table.cuda(), k_codes=codes(total, h, BLOCK, d), v_codes=codes(total, h, d, BLOCK),
+                 k_scale=torch.rand(total, h, generator=gen, device="cuda") * 0.02 + 0.02,
+                 v_scale=torch.rand(total, h, generator=gen, device="cuda") * 0.02 + 0.02)
+    # sequence and position of every new token
+    seq = torch.repeat_interleave(torch.arange(len(fresh)), torch.tensor(fresh))
+    within = torch.arange(sum(fresh)) - offsets[:-1].long()[seq]
+    state["seq"] = seq.cuda()
+    state["position"] = (torch.tensor(lengths)[seq] - torch.tensor(fresh)[seq] + within).cuda()
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    order = random.Random(seed)
+    op, s = case["op"], {}
+    if op == "rotary":
+        # q and k as they lie in the result of one fused projection, v (`other` heads) behind them
+        t, wide = case["tokens"], (case["heads"] + case["other"]) * case["head_dim"]
+        qkv = _normal(gen, t, wide)
+        w, factor = _frequencies(case)
+        s.update(case=case, t=qkv[:, :case["heads"] * case["head_dim"]].unflatten(1, (case["heads"], case["head_dim"])),
+                 positions=torch.randint(0, case["positions"], (t,), generator=gen, device="cuda", dtype=torch.int32),
+                 w=w.cuda(), factor=factor)
+        if own:
+            rotary = _framework()[0]
+            s["rotary"] = rotary.RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"], scaling=_SCALING[case["scaling"]])
+    elif op in ("append", "attend"):
+        _paged(case, gen, order, s)
+        t, h, d = sum(s["fresh"]), case["kv_heads"], case["head_dim"]
+        if op == "append":
+            kv = _normal(gen, t, 2 * h * d)
+            kv[:, h * d:] *= 0.5
+            s["k"], s["v"] = (kv[:, i * h * d:(i + 1) * h * d].unflatten(1, (h, d)) for i in (0, 1))
+            w, s["factor"] = _frequencies(case)
+            s["w"] = w.cuda()
+            s["touched"] = torch.unique(s["table"][s["seq"], s["position"] // BLOCK].long())
+        else:
+            s["q"] = _normal(gen, t, case["q_heads"], d)
+        if own:
+            rotary, kv_cache, _ = _framework()
+            s["cache"] = kv_cache.KVCacheGQ.from_tensors(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"])
+            if op == "append":
+                s["rotary"] = rotary.RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"])
+    else:
+        m, k, n, r, na = (case[x] for x in ("rows", "k", "n", "rank", "adapters"))
+        kinds = na + (1 if case["none"] else 0)
+        ids = [i * kinds // m if m >= kinds else (i * kinds + kinds // 2) // m for i in range(m)]
+        ids = [i if i < na else -1 for i in ids]
+        if not case["runs"]:
+            order.shuffle(ids)
+        s.update(case=case, ids=torch.tensor(ids, dtype=torch.int32).cuda(), x=_normal(gen, m, k),
+                 down=_normal(gen, na, r, k, std=k ** -0.5), up=_normal(gen, na, n, r, std=0.05),
+                 scaling=torch.rand(na, generator=gen, device="cuda") + 0.5)
+        if op == "adapt":
+            s["y"] = _normal(gen, m, n)
+        else:
+            s["dy"], s["dx"] = _normal(gen, m, n, std=1e-2), _normal(gen, m, k, std=1e-2)
+        if own:
+            lora = _framework()[2]
+            s["adapters"] = lora.LowRankAdapters(s["down"], s["up"], s["scaling"])
+            s["plan"] = lora.AdapterPlan(s["ids"], na)
+    return s
+
+
+# -------------------------------------------------------------------------------------------- plain forms
+
+
+def _rotated(t, position, w, factor, layout, inverse=False):
+    angle = position.double()[:, None, None] * w
+    cos, sin = (angle.cos() * factor).float(), (angle.sin() * (-factor if inverse else factor)).float()
+    r, t = 2 * w.numel(), t.float()
+    a, b = (t[..., 0:r:2], t[..., 1:r:2]) if layout == "interleaved" else (t[..., :r // 2], t[..., r // 2:r])
+    a, b = a * cos - b * sin, a * sin + b * cos
+    turned = torch.stack((a, b), -1).flatten(-2) if layout == "interleaved" else torch.cat((a, b), -1)
+    return torch.cat((turned, t[..., r:]), -1).half()
+
+
+def _quantised(x, codes, scale, block, slot, first, touched):
+    """Writes x [tokens, heads, dim] into codes [blocks, heads, BLOCK, dim] and scale [blocks, heads]; `touched`: the blocks."""
+    index = block[:, None].expand(-1, x.shape[1])
+    old = torch.where(first[:, None] > 0, scale, torch.zeros_like(scale))  # (a block that starts here has no tokens yet)
+    need = torch.zeros_like(scale).scatter_reduce(0, index, x.float().abs().amax(-1), "amax") / 127.0
+    mantissa, exponent = torch.frexp(need / old)
+    exponent = torch.where(mantissa == 0.5, exponent - 1, exponent)
+    grown = torch.where(old > 0, torch.ldexp(old, exponent), need)
+    new = torch.where(need > old, grown, old)
+    shift = torch.where(new > 0, old / new, torch.zeros_like(new))
+    kept = torch.round((codes[touched].float() - 128) * shift[touched][..., None, None]) + 128
+    codes[touched] = kept.to(torch.uint8)
+    scale[touched] = new[touched]
+    s = new[block][..., None]
+    value = torch.where(s > 0, torch.round(x.float() / s), torch.zeros_like(x, dtype=torch.float32))
+    codes[block, :, slot] = (value.clamp(-127, 127) + 128).to(torch.uint8)
+
+
+def _plain_append(s):
+    block = s["table"][s["seq"], s["position"] // BLOCK].long()
+    slot = s["position"] % BLOCK
+    # tokens that each block had before, at its first new one
+    first = torch.full((s["k_scale"].shape[0],), BLOCK, device="cuda").scatter_reduce(0, block, slot, "amin")
+    k = _rotated(s["k"], s["position"], s["w"], s["factor"], s["case"]["layout"])
+    v_codes = s["v_codes"].transpose(2, 3)
+    _quantised(k, s["k_codes"], s["k_scale"], block, slot, first, s["touched"])
+    _quantised(s["v"], v_codes, s["v_scale"], block, slot, first, s["touched"])
+    return {"k": ((s["k_codes"][block, :, slot].float() - 128) * s["k_scale"][block][..., None]).half(),
+            "v": ((v_codes[block, :, slot].float() - 128) * s["v_scale"][block][..., None]).half()}
+
+
+def _plain_attend(s):
+    b, h, d = len(s["lengths"]), s["case"]["kv_heads"], s["case"]["head_dim"]
+    group = s["case"]["q_heads"] // h
+    most, table = max(s["fresh"]), s["table"].long()
+    k = (s["k_codes"][table].float() - 128) * s["k_scale"][table][..., None, None]
+    v = (s["v_codes"][table].float() - 128) * s["v_scale"][table][..., None, None]
+    k = k.permute(0, 2, 1, 3, 4).reshape(b, h, -1, d)
+    v = v.permute(0, 2, 1, 4, 3).reshape(b, h, -1, d)
+    # rows [batch, kv head, (token, head of the group)], short sequences padded
+    within = s["position"] - (s["seq_lens"] - s["offsets"].diff())[s["seq"]]
+    q = torch.zeros(b, most, h, group, d, device="cuda")
+    q[s["seq"], within] = s["q"].float().unflatten(1, (h, group))
+    q = q.permute(0, 2, 1, 3, 4).reshape(b, h, most * group, d)
+    scores = torch.matmul(q, k.transpose(2, 3)) * d ** -0.5
+    limit = torch.zeros(b, most, dtype=torch.long, device="cuda")
+    limit[s["seq"], within] = s["position"]
+    hidden = torch.arange(k.shape[2], device="cuda") > limit.repeat_interleave(group, 1)[..., None]
+    scores.masked_fill_(hidden[:, None], -math.inf)
+    p = torch.exp(scores - scores.amax(-1, keepdim=True))
+    o = torch.matmul(p, v) / p.sum(-1, keepdim=True)
+    o = o.reshape(b, h, most, group, d).permute(0, 2, 1, 3, 4)[s["seq"], within]
+    return o.flatten(1, 2).half()
+
+
+def _chosen(s):
+    """[rows, adapters]: the scaling of each row's adapter in its column."""
+    return (s["ids"][:, None] == torch.arange(s["down"].shape[0], device="cuda")) * s["scaling"]
+
+
+def _plain_adapt(s):
+    m, (na, r, k), n = s["x"].shape[0], s["down"].shape, s["up"].shape[1]
+    v = torch.matmul(s["x"].float(), s["down"].float().reshape(na * r, k).t())
+    v = (v.reshape(m, na, r) * _chosen(s)[..., None]).reshape(m, na * r)
+    z = s["y"].float() + torch.matmul(v, s["up"].float().permute(0, 2, 1).reshape(na * r, n))
+    if s["case"]["activation"] == "relu":
+        z = z.clamp(min=0)
+    elif s["case"]["activation"] == "gelu_tanh":
+        z = 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z * z * z)))
+    return z.half()
+
+
+def _plain_adapt_back(s):
+    m, (na, r, k), n = s["x"].shape[0], s["down"].shape, s["up"].shape[1]
+    x, dy, chosen = s["x"].float(), s["dy"].float(), _chosen(s)[..., None]
+    down, up = s["down"].float().reshape(na * r, k), s["up"].float().permute(0, 2, 1).reshape(na * r, n)
+    v = (torch.matmul(x, down.t()).reshape(m, na, r) * chosen).reshape(m, na * r)
+    dv = (torch.matmul(dy, up.t()).reshape(m, na, r) * chosen).reshape(m, na * r)
+    return {"dx": (s["dx"].float() + torch.matmul(dv, down)).half(), "d_down": torch.matmul(dv.t(), x).reshape(na, r, k),
+            "d_up": torch.matmul(dy.t(), v).reshape(n, na, r).permute(1, 0, 2).contiguous()}
+
+
+def run(state):
+    s, op = state, state["case"]["op"]
+    if own:
+        rotary, kv_cache, lora = _framework()
+        if op == "rotary":
+            return rotary.rotary_pos_embed(s["t"], s["positions"], s["rotary"], inverse=s["case"]["inverse"])
+        if op == "append":
+            kv_cache.kv_cache_append(s["cache"], s["k"], s["v"], s["offsets"], s["seq_lens"], s["table"], rotary=s["rotary"])
+            k, v = kv_cache.kv_cache_gather(s["cache"], s["offsets"], s["seq_lens"], s["table"], tokens=s["k"].shape[0])
+            return {"k": k, "v": v}
+        if op == "attend":
+            return kv_cache.kv_cache_attention(s["q"], s["cache"], s["offsets"], s["seq_lens"], s["table"])
+        if op == "adapt":
+            return lora.low_rank_adapters(s["x"], s["y"], s["adapters"], s["plan"], activation=s["case"]["activation"] or None)
+        dx, d_down, d_up = lora.low_rank_adapters_grad(s["x"], s["dy"], s["adapters"], s["plan"], dx=s["dx"])
+        return {"dx": dx, "d_down": d_down, "d_up": d_up}
+    if op == "rotary":
+        return _rotated(s["t"], s["positions"], s["w"], s["factor"], s["case"]["layout"], s["case"]["inverse"])
+    return {"append": _plain_append, "attend": _plain_attend, "adapt": _plain_adapt, "adapt_back": _plain_adapt_back}[op](s)
+
+
+# ---------------------------------------------------------------------------------------------------- work
+
+
+def work(case):
+    op = case["op"]
+    if op == "rotary":
+        elements = case["tokens"] * case["heads"] * case["head_dim"]
+        return {"bytes": 4 * elements + 4 * case["tokens"], "flops": 3 * case["tokens"] * case["heads"] * case["rotary_dim"]}
+    if op in ("append", "attend"):
+        lengths, fresh = _lengths(case, random.Random(0))
+        h, d, t = case["kv_heads"], case["head_dim"], sum(fresh)
+        if op == "append":  # k and v read, their codes written, the codes read back, the values written
+            return {"bytes": t * h * d * 2 * (2 + 1 + 1 + 2), "flops": t * h * (2 * 3 * d + 3 * case["rotary_dim"])}
+        seen = sum(n * f - f * (f - 1) // 2 for n, f in zip(lengths, fresh))
+        blocks = sum(-(-n // BLOCK) for n in lengths)
+        return {"bytes": 2 * sum(lengths) * h * d + 8 * blocks * h + 4 * t * case["q_heads"] * d, "flops": 4 * seen * case["q_heads"] * d}
+    m, k, n, r = (case[x] for x in ("rows", "k", "n", "rank"))
+    kinds = case["adapters"] + (1 if case["none"] else 0)
+    used = min(m, case["adapters"])
+    with_one = m * case["adapters"] // kinds
+    if op == "adapt":
+        return {"bytes": 2 * (m * (k + 2 * n) + used * r * (k + n)), "flops": 2 * with_one * r * (k + n)}
+    return {"bytes": 2 * (m * (3 * k + n) + used * r * (k + n)) + 4 * case["adapters"] * r * (k + n), "flops": 6 * with_one * r * (k + n)}
+
+
+# --------------------------------------------------------------------------------------------------- exact
+
+
+def _exact_rotation(t, position, w, factor, layout, sign):
+    """Each pair as one complex number, turned by exp(i angle)."""
+    t = t.double().clone()
+    half = w.numel()
+    one = torch.arange(half, device="cuda") * (2 if layout == "interleaved" else 1)
+    two = one + (1 if layout == "interleaved" else half)
+    turn = torch.polar(torch.full((t.shape[0], half), factor, dtype=torch.float64, device="cuda"), sign * torch.outer(position.double(), w))
+    z = torch.complex(t[:, :, one], t[:, :, two]) * turn[:, None]
+    t[:, :, one], t[:, :, two] = z.real, z.imag
+    return t
+
+
+def exact(case, seed):
+    s, op = prepare(case, seed), case["op"]
+    if op == "rotary":
+        return _exact_rotation(s["t"], s["positions"], s["w"], s["factor"], case["layout"], -1 if case["inverse"] else 1)
+    if op == "append":
+        # What the codes stand for hangs on roundings of 32-bit scales: taken sequence by sequence, block by block.
+        turned = _exact_rotation(s["k"], s["position"], s["w"], s["factor"], case["layout"], 1).half()
+        out, at = {"k": [], "v": []}, 0
+        for b, (n, f) in enumerate(zip(s["lengths"], s["fresh"])):
+            p = n - f
+            while p < n:
+                q = min(n, (p // BLOCK + 1) * BLOCK)
+                block = int(s["table"][b, p // BLOCK])
+                for name, x, scale in (("k", turned, s["k_scale"]), ("v", s["v"], s["v_scale"])):
+                    x = x[at:at + q - p].double()
+                    need = (x.abs().amax((0, 2)).float() / 127).double()
+                    step = need
+                    if p % BLOCK:
+                        step = scale[block].double()
+                        step = torch.where(need > step, step * 2.0 ** torch.ceil(torch.log2(need / step)), step)
+                    step = step[None, :, None]
+                    out[name].append(torch.round(x / step) * step)
+                at, p = at + q - p, q
+        return {name: torch.cat(v) for name, v in out.items()}
+    if op == "attend":
+        group, d, parts, at = case["q_heads"] // case["kv_heads"], case["head_dim"], [], 0
+        for b, (n, f) in enumerate(zip(s["lengths"], s["fresh"])):
+            ids = s["table"][b, :-(-n // BLOCK)].long()
+            heads = []
+            for h in range(case["kv_heads"]):
+                k = ((s["k_codes"][ids, h].double() - 128) * s["k_scale"][ids, h].double()[:, None, None]).reshape(-1, d)[:n]
+                v = ((s["v_codes"][ids, h].double() - 128) * s["v_scale"][ids, h].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:n]
+                for g in range(group):
+                    z = s["q"][at:at + f, h * group + g].double() @ k.t() / math.sqrt(d)
+                    z += torch.full((f, n), -math.inf, dtype=torch.float64, device="cuda").triu(n - f + 1)
+                    heads.append(torch.softmax(z, -1) @ v)
+            parts.append(torch.stack(heads, 1))
+            at += f
+        return torch.cat(parts)
+    x, ids = s["x"].double(), s["ids"]
+    if op == "adapt":
+        z = s["y"].double()
+        for a in range(case["adapters"]):
+            rows = (ids == a).nonzero()[:, 0]
+            z[rows] += s["scaling"][a].double() * ((x[rows] @ s["down"][a].double().t()) @ s["up"][a].double().t())
+        if case["activation"] == "relu":
+            return torch.relu(z)
+        if case["activation"] == "gelu_tanh":
+            return torch.nn.functional.gelu(z, approximate="tanh")
+        return z
+    dx, d_down, d_up = s["dx"].double(), [], []
+    for a in range(case["adapters"]):
+        rows = (ids == a).nonzero()[:, 0]
+        xa, dy, scale = x[rows], s["dy"][rows].double(), s["scaling"][a].double()
+        down, up = s["down"][a].double(), s["up"][a].double()
+        dx[rows] += scale * (dy @ up) @ down
+        d_down.append(scale * (dy @ up).t() @ xa)
+        d_up.append(scale * dy.t() @ (xa @ down.t()))
+    return {"dx": dx, "d_down": torch.stack(d_down), "d_up": torch.stack(d_up)}
