@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define GQ_ABI_VERSION 4
+#define GQ_ABI_VERSION 5
 
 #define GQ_OK 0
 #define GQ_ERR_NULL_POINTER (-1) /* a required pointer is NULL */
@@ -409,6 +409,113 @@ int gq_compress_f16(const uint16_t *t, uint16_t *packed, uint16_t *scale, uint16
 int gq_compress_f32(const float *t, uint16_t *packed, uint16_t *scale, uint16_t *bias,
                     int32_t *nonfinite_flag, int64_t rows, int64_t n_groups, int64_t group_size,
                     void *stream);
+
+/*
+ * Operators that a decoder needs beside its 4-bit projections.  No counterpart in the reference's binding.
+ *
+ * Rotary positions.  Pair i (i < rotary_dim / 2) of a row is turned by 2 pi positions[token] turns[i]:
+ *   (a, b) -> factor (a cos - b sin, a sin + b cos);  inverse: by the opposite angle, which gives the gradient.
+ * GQ_ROTARY_INTERLEAVED: the pair is elements 2i and 2i + 1;  GQ_ROTARY_HALF: elements i and i + rotary_dim / 2.  Elements
+ * behind rotary_dim are copied.  The angle is formed in binary64, so positions may be any int32.
+ *   t, out     [tokens, heads, head_dim] binary16, the last axis contiguous, strides in elements; out may be t (same strides),
+ *              other overlaps are the caller's error
+ *   positions  [tokens] int32;  turns [rotary_dim / 2] binary64
+ * rotary_dim is even and <= 256.  The fast kernel needs 16-byte aligned rows (strides and head_dim % 8 == 0) and rotary_dim % 8
+ * (interleaved) or % 16 (half); others run element by element with the same results.
+ */
+#define GQ_ROTARY_INTERLEAVED 0
+#define GQ_ROTARY_HALF 1
+typedef struct gq_rotary {
+  const double *turns; /* device, [rotary_dim / 2]: turns a position */
+  float factor;        /* of the turned pairs (1, or the attention factor of a stretched context) */
+  int32_t rotary_dim;
+  int32_t layout;      /* GQ_ROTARY_* */
+} gq_rotary;
+int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stride, const int32_t *positions,
+                  const gq_rotary *rotary, int32_t inverse, uint16_t *out, int64_t out_token_stride, int64_t out_head_stride,
+                  int64_t tokens, int64_t heads, int64_t head_dim, void *stream);
+
+/*
+ * 8-bit key/value cache in blocks of GQ_KV_BLOCK tokens, one binary32 scale for the keys and one for the values of each
+ * (block, head); value = (byte - 128) * scale, bytes 1 ... 255.  head_dim is a multiple of 16, at most 256; the code arrays are
+ * 16-byte aligned.
+ *
+ * A batch is B sequences.  Rows offsets[b] ... offsets[b + 1] - 1 of the row tensors (k, v, q, out) are the newest tokens of
+ * sequence b, seq_lens[b] its length with them: its last row has position seq_lens[b] - 1.  A sequence that is given more rows
+ * than it has tokens is padded in front: those rows are not stored and attend to nothing (zeros).  Token t of sequence b lies in
+ * block block_table[b][t / GQ_KV_BLOCK]; no two sequences of a batch may append to the same block.  offsets ascend from 0;
+ * rows from offsets[B] on are neither read nor written.  These arrays are device data that no call waits for: a length beyond
+ * the table's width is cut to it, and a block number outside [0, n_blocks) is a block that is not there -- nothing is stored
+ * in it, nothing read back from it, and attention passes over its tokens.
+ *
+ * gq_kv_append_f16     stores k and v [tokens, kv_heads, head_dim] (strides in elements, multiples of 8; 16-byte aligned), the
+ *   keys turned first if `rotary` is not NULL (rotary_dim % 8 == 0, half layout % 16; rounded to binary16 as gq_rotary_f16
+ *   does).  A block that starts with these tokens gets scale amax / 127; in one that has tokens the scale grows, where it
+ *   must, by a power of two and the codes there are scaled down by it: |value - x| < scale always.  A value that is not
+ *   finite makes all values of its (block, head) not finite.
+ * gq_kv_gather_f16     the values of the batch's rows, [tokens, kv_heads, head_dim] binary16, contiguous, 16-byte aligned.
+ * gq_kv_attention_f16  out[row][head] = softmax(scale q . k) v over the tokens at the row's position and before, query head i
+ *   with kv head i / (q_heads / kv_heads).  q, out [tokens, q_heads, head_dim]: q strides multiples of 8 and 16-byte aligned,
+ *   out any strides (elements).  Binary32 softmax and sums; probabilities enter the product with the values as binary16.
+ *   workspace: gq_kv_attention_workspace_bytes() bytes, 16-byte aligned, any contents, not shared by calls that may overlap.
+ */
+#define GQ_KV_BLOCK 64
+typedef struct gq_kv_cache {
+  uint8_t *k_codes; /* [n_blocks][kv_heads][GQ_KV_BLOCK][head_dim] */
+  uint8_t *v_codes; /* [n_blocks][kv_heads][head_dim][GQ_KV_BLOCK] */
+  float *k_scale;   /* [n_blocks][kv_heads] */
+  float *v_scale;
+  int64_t n_blocks;
+  int32_t kv_heads, head_dim;
+} gq_kv_cache;
+typedef struct gq_kv_batch {
+  const int32_t *offsets;     /* [sequences + 1] */
+  const int32_t *seq_lens;    /* [sequences] */
+  const int32_t *block_table; /* [sequences][table_width] */
+  int64_t sequences, table_width;
+  int64_t tokens;             /* rows of the row tensors */
+} gq_kv_batch;
+int gq_kv_append_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, const uint16_t *k, int64_t k_token_stride,
+                     int64_t k_head_stride, const uint16_t *v, int64_t v_token_stride, int64_t v_head_stride,
+                     const gq_rotary *rotary, void *stream);
+int gq_kv_gather_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, uint16_t *k, uint16_t *v, void *stream);
+int64_t gq_kv_attention_workspace_bytes(int64_t head_dim);
+int gq_kv_attention_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, const uint16_t *q, int64_t q_token_stride,
+                        int64_t q_head_stride, uint16_t *out, int64_t out_token_stride, int64_t out_head_stride,
+                        int64_t q_heads, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection: row m has adapter a = ids[m], and
+ *   out[m] = act(y[m] + scaling[a] (x[m] down[a]^T) up[a]^T);   rows whose id is outside [0, n_adapters): act(y[m])
+ * 1 <= rank <= 128, n_adapters <= 2048, rows <= 2^24.  Sums are binary32, x down^T is kept in binary32.
+ *
+ * gq_adapter_plan        sorts a batch's rows by adapter, on the device; the plan (gq_adapter_plan_bytes() bytes, 16-byte
+ *   aligned) serves every projection of the batch until the ids change.
+ * gq_adapter_apply_f16   x [rows, in], y and out [rows, out] (row strides in elements; y == NULL: zeros; out may be y with the
+ *   same stride).  The fast kernels need 16-byte aligned rows and rank % 8 == 0.
+ * gq_adapter_grad_f16    from dy = dL/dout (no activation): dx_out = dx + scaling dy up down (dx == NULL: zeros; dx_out may be
+ *   dx with the same stride), d_down [n_adapters, rank, in] and d_up [n_adapters, out, rank] in binary32, zeros for
+ *   adapters without rows.
+ * Each workspace: the matching size function's bytes, 256-byte aligned, any contents, not shared by calls that may overlap.
+ * The order of every sum is fixed by the sizes and ids: equal calls give equal bits.
+ */
+typedef struct gq_adapters {
+  const uint16_t *down;  /* [n_adapters, rank, in_features] binary16 */
+  const uint16_t *up;    /* [n_adapters, out_features, rank] binary16 */
+  const float *scaling;  /* [n_adapters] */
+  int64_t n_adapters, rank, in_features, out_features;
+} gq_adapters;
+int64_t gq_adapter_plan_bytes(int64_t rows, int64_t n_adapters);
+int gq_adapter_plan(const int32_t *ids, int64_t rows, int64_t n_adapters, void *plan, int64_t plan_bytes, void *stream);
+int64_t gq_adapter_apply_workspace_bytes(const gq_adapters *adapters, int64_t rows);
+int gq_adapter_apply_f16(const gq_adapters *adapters, const void *plan, int64_t rows, const uint16_t *x, int64_t x_row_stride,
+                         const uint16_t *y, int64_t y_row_stride, uint16_t *out, int64_t out_row_stride, int32_t activation,
+                         void *workspace, int64_t workspace_bytes, void *stream);
+int64_t gq_adapter_grad_workspace_bytes(const gq_adapters *adapters, int64_t rows);
+int gq_adapter_grad_f16(const gq_adapters *adapters, const void *plan, int64_t rows, const uint16_t *x, int64_t x_row_stride,
+                        const uint16_t *dy, int64_t dy_row_stride, const uint16_t *dx, int64_t dx_row_stride, uint16_t *dx_out,
+                        int64_t dx_out_row_stride, float *d_down, float *d_up, void *workspace, int64_t workspace_bytes,
+                        void *stream);
 
 #ifdef __cplusplus
 }

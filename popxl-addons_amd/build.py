@@ -19,7 +19,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libgq_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["gq_api.hip", "gq_decompress.hip", "gq_compress.hip", "gq_gemv.hip", "gq_gemv_stream.hip", "gq_gemv_flow.hip", "gq_gemm.hip", "gq_linear_kn.hip",
-           "gq_gemv_kn.hip", "gq_gemv_sums.hip", "gq_gemv_rows.hip"]
+           "gq_gemv_kn.hip", "gq_gemv_sums.hip", "gq_gemv_rows.hip",
+           "gq_api_operators.hip", "gq_rotary.hip", "gq_kv_cache.hip", "gq_kv_attention.hip", "gq_adapters.hip"]
 
 # -ffp-contract=off: the decompress contract is "fp16 multiply, then fp16 add" (two roundings);
 # kernels that want an fma ask for one explicitly.  Packed-fp32 instruction selection is disabled.

@@ -111,5 +111,27 @@ int launch_compress(const uint16_t *t, uint16_t *packed, uint16_t *scale, uint16
                     int64_t rows, int64_t n_groups, int64_t group_size, hipStream_t stream);
 int launch_compress_f32(const float *t, uint16_t *packed, uint16_t *scale, uint16_t *bias, int32_t *flag,
                         int64_t rows, int64_t n_groups, int64_t group_size, hipStream_t stream);
+// Operators beside the projections (gq_rotary.hip, gq_kv_cache.hip, gq_kv_attention.hip, gq_adapters.hip)
+struct KvCache;
+struct KvBatch;
+int launch_rotary(const uint16_t *t, int64_t t_token, int64_t t_head, const int32_t *positions, const gq_rotary &rotary,
+                  bool inverse, uint16_t *out, int64_t o_token, int64_t o_head, int64_t tokens, int64_t heads,
+                  int64_t head_dim, hipStream_t stream);
+int launch_kv_append(const KvCache &cache, const KvBatch &batch, const uint16_t *k, int64_t k_token, int64_t k_head,
+                     const uint16_t *v, int64_t v_token, int64_t v_head, const gq_rotary *rotary, hipStream_t stream);
+int launch_kv_gather(const KvCache &cache, const KvBatch &batch, uint16_t *k, uint16_t *v, hipStream_t stream);
+int64_t kv_attention_workspace_bytes(int64_t dim);
+int launch_kv_attention(const KvCache &cache, const KvBatch &batch, const uint16_t *q, int64_t q_token, int64_t q_head,
+                        uint16_t *out, int64_t o_token, int64_t o_head, int64_t q_heads, float scale, void *workspace,
+                        hipStream_t stream);
+int64_t adapter_plan_bytes(int64_t rows, int64_t adapters);
+int launch_adapter_plan(const int32_t *ids, int64_t rows, int64_t adapters, void *plan, hipStream_t stream);
+int64_t adapter_apply_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t rank);
+int launch_adapter_apply(const gq_adapters &w, const void *plan, int64_t rows, const uint16_t *x, int64_t x_stride, const uint16_t *y,
+                         int64_t y_stride, uint16_t *out, int64_t out_stride, int act, void *workspace, hipStream_t stream);
+int64_t adapter_grad_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t out, int64_t rank);
+int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, const uint16_t *x, int64_t x_stride, const uint16_t *dy,
+                        int64_t dy_stride, const uint16_t *dx, int64_t dx_stride, uint16_t *dx_out, int64_t dx_out_stride, float *d_down,
+                        float *d_up, void *workspace, hipStream_t stream);
 
 }  // namespace gq

@@ -10,13 +10,14 @@ import os
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 _DEFAULT_LIB = os.path.join(os.path.dirname(_PKG_DIR), "lib", "libgq_hip.so")
 
-GQ_ABI_VERSION = 4
+GQ_ABI_VERSION = 5
 GQ_ERR_NULL_POINTER = -1
 GQ_ERR_BAD_SHAPE = -2
 GQ_ERR_MISALIGNED = -3
 GQ_ERR_UNSUPPORTED = -4
 GQ_ERR_NO_DEVICE = -5
 GQ_ACT_NONE, GQ_ACT_RELU, GQ_ACT_GELU_TANH = 0, 1, 2
+GQ_ROTARY_INTERLEAVED, GQ_ROTARY_HALF = 0, 1
 GQ_DESC_KN_LAYOUT = 0x100  # or-ed into a sequence entry's activation: weight grouped along the output features
 ACTIVATIONS = {None: GQ_ACT_NONE, "none": GQ_ACT_NONE, "relu": GQ_ACT_RELU, "gelu_tanh": GQ_ACT_GELU_TANH}
 
@@ -58,7 +59,37 @@ EXPORTS = (
     "gq_linear_knp_strided_f16",
     "gq_compress_f16",
     "gq_compress_f32",
+    "gq_rotary_f16",
+    "gq_kv_append_f16",
+    "gq_kv_gather_f16",
+    "gq_kv_attention_workspace_bytes",
+    "gq_kv_attention_f16",
+    "gq_adapter_plan_bytes",
+    "gq_adapter_plan",
+    "gq_adapter_apply_workspace_bytes",
+    "gq_adapter_apply_f16",
+    "gq_adapter_grad_workspace_bytes",
+    "gq_adapter_grad_f16",
 )
+
+
+class Rotary(ctypes.Structure):  # gq_rotary
+    _fields_ = [("turns", ctypes.c_void_p), ("factor", ctypes.c_float), ("rotary_dim", ctypes.c_int32), ("layout", ctypes.c_int32)]
+
+
+class KvCache(ctypes.Structure):  # gq_kv_cache
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("n_blocks", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class KvBatch(ctypes.Structure):  # gq_kv_batch
+    _fields_ = [("offsets", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("sequences", ctypes.c_int64), ("table_width", ctypes.c_int64), ("tokens", ctypes.c_int64)]
+
+
+class Adapters(ctypes.Structure):  # gq_adapters
+    _fields_ = [("down", ctypes.c_void_p), ("up", ctypes.c_void_p), ("scaling", ctypes.c_void_p), ("n_adapters", ctypes.c_int64),
+                ("rank", ctypes.c_int64), ("in_features", ctypes.c_int64), ("out_features", ctypes.c_int64)]
 
 
 class GQHipError(RuntimeError):
@@ -140,6 +171,22 @@ def load():
         fn = getattr(lib, name)
         fn.argtypes = [p, p, p, p, p, i64, i64, i64, p]
         fn.restype = ctypes.c_int
+    i32, f32 = ctypes.c_int32, ctypes.c_float
+    for name, result, arguments in (
+        ("gq_rotary_f16", ctypes.c_int, [p, i64, i64, p, p, i32, p, i64, i64, i64, i64, i64, p]),
+        ("gq_kv_append_f16", ctypes.c_int, [p, p, p, i64, i64, p, i64, i64, p, p]),
+        ("gq_kv_gather_f16", ctypes.c_int, [p, p, p, p, p]),
+        ("gq_kv_attention_workspace_bytes", i64, [i64]),
+        ("gq_kv_attention_f16", ctypes.c_int, [p, p, p, i64, i64, p, i64, i64, i64, f32, p, i64, p]),
+        ("gq_adapter_plan_bytes", i64, [i64, i64]),
+        ("gq_adapter_plan", ctypes.c_int, [p, i64, i64, p, i64, p]),
+        ("gq_adapter_apply_workspace_bytes", i64, [p, i64]),
+        ("gq_adapter_apply_f16", ctypes.c_int, [p, p, i64, p, i64, p, i64, p, i64, i32, p, i64, p]),
+        ("gq_adapter_grad_workspace_bytes", i64, [p, i64]),
+        ("gq_adapter_grad_f16", ctypes.c_int, [p, p, i64, p, i64, p, i64, p, i64, p, i64, p, p, p, i64, p]),
+    ):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = result, arguments
     if lib.gq_abi_version() != GQ_ABI_VERSION:
         raise ImportError(f"{path}: ABI version {lib.gq_abi_version()} != expected {GQ_ABI_VERSION}")
     _lib = lib

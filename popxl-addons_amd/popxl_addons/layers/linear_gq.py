@@ -10,6 +10,7 @@ from popxl_addons.ops.group_quantize_decompress import (
     group_quantize_compress,
     group_quantize_compress_numpy,
 )
+from popxl_addons.ops.low_rank_adapters import low_rank_adapters, low_rank_adapters_grad
 from popxl_addons.utils import NamedTensors, Variable, WeightsDict, _numpy_dtype_of
 
 
@@ -104,14 +105,23 @@ class LinearGQ:
 
     # --------------------------------------------------------------------------------- build
 
-    def build(self, x, activation=None):
+    def build(self, x, activation=None, adapters=None, plan=None):
         """y = x @ decompress(weight) (+ bias), linear_gq.py:99-109.  x: float16 [..., in] on the GPU.
 
         activation (None, "relu", "gelu_tanh") is an addition to the reference's signature: the
-        epilogue is fused into the kernel."""
+        epilogue is fused into the kernel.  So are adapters (a LowRankAdapters of this layer's sizes) and
+        plan (the AdapterPlan of x's rows): y = act(x @ w + bias + the row's low-rank adapter)."""
         import torch
 
         act = _gq_hip.activation_code(activation)
+        if (adapters is None) != (plan is None):
+            raise ValueError("LinearGQ: adapters and plan go together")
+        if adapters is not None:
+            if (adapters.in_features, adapters.out_features) != (x.shape[-1], self.out_features):
+                raise ValueError(f"LinearGQ: the adapters are {adapters.in_features} -> {adapters.out_features}, the layer "
+                                 f"{x.shape[-1]} -> {self.out_features}")
+            y = self.build(x)
+            return low_rank_adapters(x, y, adapters, plan, activation=act, out=y)
 
         if not x.is_cuda:
             raise RuntimeError("LinearGQ runs on the GPU only: move x to a HIP device")
@@ -176,6 +186,46 @@ class LinearGQ:
         return y.reshape(*x.shape[:-1], self.out_features)
 
     __call__ = build
+
+    def grad(self, dy, x=None, adapters=None, plan=None):
+        """Gradients of `build` without an activation, for dy = dL/dy float16 [..., out]: an addition to the reference, whose
+        packed weight takes no gradient either.  Returns dL/dx = dy @ decompress(weight)^T, through the fused kernels of the
+        other layout (the weight's rows are features of dy where those of `build` are features of x); with adapters, plan and
+        the x of `build`: (dL/dx, d_down, d_up) as `low_rank_adapters_grad` returns them."""
+        import torch
+
+        if self.variables is None:
+            raise ValueError("LinearGQ.grad: the layer has no variables yet (build it or call init_variables)")
+        if not dy.is_cuda:
+            raise RuntimeError("LinearGQ runs on the GPU only: move dy to a HIP device")
+        v = self.variables
+        if dy.dtype != torch.float16 or v.weight_decompression_scale.dtype != torch.float16:
+            raise TypeError("LinearGQ: only float16 activations and float16 scale/bias are supported")
+        if dy.shape[-1] != self.out_features:
+            raise ValueError(f"LinearGQ.grad: dy has {dy.shape[-1]} features, the layer {self.out_features}")
+        if (adapters is None) != (plan is None) or (adapters is None) != (x is None):
+            raise ValueError("LinearGQ.grad: x, adapters and plan go together")
+        rows, n_groups, _ = v.weight_compressed.shape
+        in_features = n_groups * self.group_size if self.dim == 0 else rows
+        if adapters is not None and (adapters.in_features, adapters.out_features) != (in_features, self.out_features):
+            raise ValueError(f"LinearGQ.grad: the adapters are {adapters.in_features} -> {adapters.out_features}, the layer "
+                             f"{in_features} -> {self.out_features}")
+        if x is not None and tuple(x.shape) != (*dy.shape[:-1], in_features):
+            raise ValueError(f"LinearGQ.grad: x has shape {tuple(x.shape)}, expected {(*dy.shape[:-1], in_features)}")
+        dy2 = dy.reshape(-1, self.out_features).contiguous()
+        m_rows = dy2.shape[0]
+        with torch.cuda.device(dy.device):
+            dx = torch.empty((m_rows, in_features), dtype=torch.float16, device=dy.device)
+            name, need_of = ("gq_linear_kn_act_f16", "gq_linear_kn_workspace_bytes") if self.dim == 0 else (
+                "gq_linear_act_ws_f16", "gq_gemm_workspace_bytes")
+            need = getattr(_gq_hip.load(), need_of)(m_rows, in_features, self.out_features, self.group_size)
+            ws = _gq_hip.linear_kn_workspace(dy.device, need) if need > 0 else None
+            _gq_hip.call(name, dy2.data_ptr(), m_rows, v.weight_compressed.data.data_ptr(), v.weight_decompression_scale.data.data_ptr(),
+                         v.weight_decompression_bias.data.data_ptr(), 0, dx.data_ptr(), in_features, self.out_features,
+                         self.group_size, _gq_hip.GQ_ACT_NONE, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                         torch.cuda.current_stream(dy.device).cuda_stream)
+        dx = dx.reshape(*dy.shape[:-1], in_features)
+        return dx if adapters is None else low_rank_adapters_grad(x, dy, adapters, plan, dx=dx)
 
     # ------------------------------------------------------------------------------- fusion
 
