@@ -5,14 +5,15 @@
 namespace gq {
 
 constexpr int kAdapterSmallTile = 16, kAdapterLargeTile = 64;  // rows of one adapter that a workgroup takes together
-constexpr int kAdapterSegment = 512;                           // rows that one part of a weight gradient sums over
+constexpr int kAdapterSegment = 2048;                          // rows that one part of a weight gradient sums over
 constexpr int kMostAdapters = 2048;
 constexpr int64_t kMostAdapterRows = (int64_t)1 << 24;
 
 struct AdapterTile {
   int adapter;  // -1: rows without one
   int begin, count;
-  int part;  // segments: the part it writes, -1 where it is its adapter's only one
+  int first;  // segments: where its tiles begin in the list of small ones (small tiles) and of large ones, and
+  int first_large, part, spare;  // the part it writes, -1 where it is its adapter's only one
 };
 
 // Where the arrays of a plan lie (4-byte words from its start).  Sizes depend on the numbers of rows and adapters alone;
@@ -25,7 +26,7 @@ struct PlanLayout {
     const int64_t kinds = rows < adapters + 1 ? rows : adapters + 1;
     most_small = rows / kAdapterSmallTile + kinds, most_large = rows / kAdapterLargeTile + kinds;
     most_segments = rows / kAdapterSegment + kinds;
-    most_parts = 2 * rows / kAdapterSegment;  // an adapter of s >= 2 segments has more than 512 (s - 1) >= 256 s rows
+    most_parts = 2 * rows / kAdapterSegment;  // an adapter of s >= 2 segments has more than 2048 (s - 1) >= 1024 s rows
     int64_t at = 0;
     const auto take = [&](int64_t n) {
       const int64_t here = at;
@@ -35,7 +36,7 @@ struct PlanLayout {
     counts = take(64);               // small tiles, large tiles, segments, parts
     order = take(rows);              // the rows, by adapter and then by index; those without one last
     parts = take(2 * adapters);      // of each adapter: its first part, its segments
-    small = take(4 * most_small), large = take(4 * most_large), segments = take(4 * most_segments);
+    small = take(8 * most_small), large = take(8 * most_large), segments = take(8 * most_segments);
     words = at;
   }
 };

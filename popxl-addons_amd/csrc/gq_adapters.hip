@@ -5,8 +5,8 @@
 //                      adapter, so that each product below is a plain matrix product over gathered rows.
 // adapter_down_kernel  v = x A^T (contraction over the features): a split of the features per workgroup, binary32 parts.
 // adapter_up_kernel    y' = act(y + s v B^T) (contraction over the rank).
-//   The gradients are the same two products with the weights turned (`kTurned`: through LDS): dv = dy B, dx' = dx + s dv A, and
-// adapter_outer_kernel dA = s dv^T x, dB = s dy^T v (contraction over rows; parts of 512 rows, added in order by
+//   The gradients are the same two products with the weights turned (adapter_turn_kernel): dv = dy B, dx' = dx + s dv A, and
+// adapter_outer_kernel dA = s dv^T x, dB = s dy^T v (contraction over rows; parts of 2048 rows, added in order by
 //                      adapter_sum_kernel; no atomics anywhere, so results do not depend on timing).
 //
 // v is held in 32 bits.  Where it enters a second product it is split into two binary16 numbers, v = hi + lo, after a power of
@@ -121,17 +121,18 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
   for (int e = 0; e < kEach; ++e) {
     const int kind = tid * each + e;
     if (e >= each || kind >= kinds) continue;
-    const int adapter = kind < a.adapters ? kind : -1, n = total[e], begin = before[0];
+    const int adapter = kind < a.adapters ? kind : -1, n = total[e], begin = before[0], small = before[1], large = before[2];
     for (int i = 0; i < n; i += kAdapterSmallTile)
-      ((AdapterTile *)(a.plan + a.small))[before[1]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterSmallTile), -1};
+      ((AdapterTile *)(a.plan + a.small))[before[1]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterSmallTile)};
     for (int i = 0; i < n; i += kAdapterLargeTile)
-      ((AdapterTile *)(a.plan + a.large))[before[2]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterLargeTile), -1};
+      ((AdapterTile *)(a.plan + a.large))[before[2]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterLargeTile)};
     if (adapter >= 0) {
       const int segments = (n + kAdapterSegment - 1) / kAdapterSegment;
       a.plan[a.parts + 2 * kind] = part, a.plan[a.parts + 2 * kind + 1] = segments;
       for (int i = 0; i < n; i += kAdapterSegment)
         ((AdapterTile *)(a.plan + a.segments))[before[3]++] =
-            AdapterTile{adapter, begin + i, min(n - i, kAdapterSegment), segments > 1 ? part + i / kAdapterSegment : -1};
+            AdapterTile{adapter, begin + i, min(n - i, kAdapterSegment), small + i / kAdapterSmallTile, large + i / kAdapterLargeTile,
+                        segments > 1 ? part + i / kAdapterSegment : -1};
       if (segments > 1) part += segments;
     }
     int at = begin;
@@ -176,106 +177,119 @@ __device__ __forceinline__ half8_t load8(const half_t *p, int64_t valid) {
   return v;
 }
 
-// Orders a wave's own LDS stores and loads (it does not share the piece with other waves, so no barrier).
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_wave_barrier();
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-}
-
-__device__ __forceinline__ uint32_t pair_of(half_t a, half_t b) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+// The same where the other operand is zero at values that do not exist: row[at ... at + 7] of a row of `size`, or others of it.
+template <bool kWide>
+__device__ __forceinline__ half8_t load8_any(const half_t *row, int64_t at, int64_t size) {
+  if (kWide) return *(const half8_t *)(row + min(at, size - 8));
+  return load8<false>(row + at, size - at);
 }
 
 struct DownArgs {
-  const half_t *x, *w;  // w: [adapters][rank][features], turned: [adapters][features][rank]
+  const half_t *x, *w;  // w: [adapters][rank][features]
   int64_t x_stride;
   const AdapterTile *tiles;
   const int *tile_count, *order;
-  float *v;  // [splits][rows][kRank]
-  int64_t rows, features, split;  // features of one split, a multiple of 512
-  int rank;
+  float *v;     // [splits][rows][kRank]
+  float *most;  // [splits][tiles]: largest magnitudes (NULL: nobody asks)
+  int64_t rows, features, split;  // features of one split, a multiple of 128
+  int rank, most_tiles;
 };
 
-constexpr int kStep = 128;           // features that a wave takes at a time
-constexpr int kTurnedRow = kStep + 8;  // binary16 a row of a turned piece in LDS: 16-byte rows, 4 banks apart
-
-// kRank: rank rounded up to 32, 64 or 128; kTiles x 16 rows.  Wave w of a workgroup takes features 128 w + 512 i ... of the
-// workgroup's split; the four binary32 sums meet in LDS.  v^T = A x^T: a lane ends with 4 consecutive ranks of one row.
-template <int kRank, int kTiles, bool kWide, bool kTurned>
-__global__ __launch_bounds__(kThreads) void adapter_down_kernel(DownArgs a) {
+// kRank: rank rounded up to 32, 64 or 128; kTiles x 16 rows.  The four waves of a workgroup have a quarter of its features
+// each, their binary32 sums meet in LDS.  v^T = A x^T: a lane ends with 4 consecutive ranks of one row.  The operands of the
+// next 64 features are loaded before this step's products: a wave has little else to hide the latency with.
+template <int kRank, int kTiles, bool kWide>
+__global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_down_kernel(DownArgs a) {
   constexpr int kRankTiles = kRank / 16;
   extern __shared__ float shared[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
   if ((int)blockIdx.x >= *a.tile_count) return;
   const AdapterTile tile = a.tiles[blockIdx.x];
   if (tile.adapter < 0) return;
-  const int64_t from = blockIdx.y * a.split, to = min(a.features, from + a.split);
+  const int64_t mine = a.split / kWaves, from = min(a.features, blockIdx.y * a.split + wave * mine), to = min(a.features, from + mine);
   const half_t *w = a.w + (int64_t)tile.adapter * a.rank * a.features;
-  const half_t *x[kTiles];
+  const half_t *x[kTiles], *wr[kRankTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) x[t] = a.x + (int64_t)a.order[tile.begin + min(t * 16 + m, tile.count - 1)] * a.x_stride;
-  half_t *turned = (half_t *)shared + wave * kRank * kTurnedRow;
+#pragma unroll
+  for (int r = 0; r < kRankTiles; ++r) wr[r] = w + (int64_t)min(r * 16 + m, a.rank - 1) * a.features;
 
   float4_t acc[kRankTiles][kTiles];
 #pragma unroll
   for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) acc[r][t] = float4_t{};
-  for (int64_t k0 = from + wave * kStep; k0 < to; k0 += kWaves * kStep) {
-    if (kTurned) {
-      // this wave's piece [128 features][rank] to [rank][features]: two features' 8 ranks at a time, 4-byte stores
-      const int columns = (a.rank + 7) / 8;
-      for (int n = lane; n < kStep / 2 * columns; n += 64) {
-        const int c = n % columns, f = n / columns * 2;
-        const half_t *p = w + (k0 + f) * a.rank + c * 8;
-        const int64_t left = a.rank - c * 8;
-        const half8_t u0 = load8<kWide>(p, k0 + f < to ? left : 0), u1 = load8<kWide>(p + a.rank, k0 + f + 1 < to ? left : 0);
+  // 64 features a step: a lane has 16 consecutive ones of a row (both operands agree on which), so that a row's 128 bytes are
+  // asked for together
+  half8_t xf[2][kTiles][2], wf[2][kRankTiles][2];
+  const auto load = [&](int set, int64_t k) {
+    k += g * 16;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *(uint32_t *)(turned + (c * 8 + j) * kTurnedRow + f) = pair_of(u0[j], u1[j]);
-      }
-      wave_lds_fence();
-    }
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int s = 0; s < kStep / 32; ++s) {
-      const int64_t k = k0 + s * 32 + g * 8;
-      half8_t xf[kTiles];
+      for (int u = 0; u < 2; ++u) xf[set][t][u] = load8<kWide>(x[t] + k + 8 * u, to - k - 8 * u);
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) xf[t] = load8<kWide>(x[t] + k, to - k);
+    for (int r = 0; r < kRankTiles; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (r * 16 < a.rank) wf[set][r][u] = load8_any<kWide>(wr[r], k + 8 * u, a.features);
+  };
+  const auto multiply = [&](int set) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < kRankTiles; ++r) {
         if (r * 16 >= a.rank) continue;
-        half8_t wf;
-        if (kTurned)
-          wf = *(const half8_t *)(turned + min(r * 16 + m, (a.rank + 7) / 8 * 8 - 1) * kTurnedRow + s * 32 + g * 8);
-        else
-          wf = load8<kWide>(w + (int64_t)min(r * 16 + m, a.rank - 1) * a.features + k, to - k);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, xf[t], acc[r][t], 0, 0, 0);
+        for (int t = 0; t < kTiles; ++t)
+          acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[set][r][u], xf[set][t][u], acc[r][t], 0, 0, 0);
       }
-    }
-    if (kTurned) wave_lds_fence();
+  };
+  if (from < to) load(0, from);
+  for (int64_t k = from; k < to; k += 128) {
+    if (k + 64 < to) load(1, k + 64);
+    multiply(0);
+    if (k + 64 >= to) break;
+    if (k + 128 < to) load(0, k + 128);
+    multiply(1);
   }
-  // sum of the four waves, 64 rows at most: [waves][16 rows][kRank + 4]
+  // sum of the four waves, 16 rows at a time: [waves][16 rows][kRank + 4]
   float *v = a.v + ((int64_t)blockIdx.y * a.rows + tile.begin) * kRank;
+  float most = 0.f;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
+    if (t * 16 >= tile.count) break;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) *(float4_t *)(shared + (wave * 16 + m) * (kRank + 4) + r * 16 + 4 * g) = acc[r][t];
     __syncthreads();
-    for (int n = threadIdx.x; n < 16 * kRank; n += kThreads) {
-      const int row = n / kRank, r = n % kRank;
-      float sum = 0.f;
+    for (int n = threadIdx.x; n < 4 * kRank; n += kThreads) {
+      const int row = n / (kRank / 4), r = n % (kRank / 4) * 4;
+      float4_t sum = {};
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) sum += shared[(i * 16 + row) * (kRank + 4) + r];
-      if (t * 16 + row < tile.count) v[(int64_t)(t * 16 + row) * kRank + r] = r < a.rank ? sum : 0.f;
+      for (int i = 0; i < kWaves; ++i) sum += *(const float4_t *)(shared + (i * 16 + row) * (kRank + 4) + r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (r + j >= a.rank) sum[j] = 0.f;
+        if (t * 16 + row < tile.count) most = fmaxf(most, fabsf(sum[j]));
+      }
+      if (t * 16 + row < tile.count) *(float4_t *)(v + (int64_t)(t * 16 + row) * kRank + r) = sum;
     }
+  }
+  if (a.most) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    __syncthreads();
+    if (lane == 0) shared[wave] = most;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      a.most[(int64_t)blockIdx.y * a.most_tiles + blockIdx.x] = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
   }
 }
 
 struct UpArgs {
-  const float *v;  // [splits][rows][kRank]
-  const half_t *w;  // [adapters][features][rank], turned: [adapters][rank][features]
+  const float *v;   // [splits][rows][kRank]
+  const half_t *w;  // [adapters][features][rank]
   const float *scaling;
   const half_t *y;  // NULL: zeros
   half_t *out;
@@ -302,12 +316,29 @@ __device__ __forceinline__ float normal_power(float most, float &back) {
   return ldexpf(1.f, -e);
 }
 
-// Wave w takes 64 features at a time: row 4 g' + i of operand tile t is feature 16 g' + 4 t + i, so that a lane ends with 16
-// consecutive features of one row (two 16-byte loads and stores, 128 bytes a row for the wave).
-template <int kRank, int kTiles, bool kWide, bool kTurned>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(UpArgs a) {
-  constexpr int kChunks = kRank / 32, kRow = kRank + 8;
-  extern __shared__ float shared[];
+// v summed over the splits, `p` a row's 4 ranks: four loads in flight
+__device__ __forceinline__ float4_t sum_of_splits(const float *p, int64_t stride, int splits) {
+  float4_t sum = {};
+  int s = 0;
+  for (; s + 4 <= splits; s += 4) {
+    float4_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = *(const float4_t *)(p + (s + i) * stride);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += u[i];
+  }
+  for (; s < splits; ++s) sum += *(const float4_t *)(p + s * stride);
+  return sum;
+}
+
+// The workgroup sums its rows' v over the splits into LDS, where its waves take their operands from.  Then wave w takes 64
+// features at a time: row 4 g' + i of operand tile f is feature 16 g' + 4 f + i, so that a lane ends with 16 consecutive
+// features of one row (two 16-byte loads and stores, 128 bytes a row for the wave).  The weights and y of the next
+// piece are loaded before and among this one's products.
+template <int kRank, int kTiles, bool kWide>
+__global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
+  constexpr int kChunks = kRank / 32, kRow = kRank + 4;
+  __shared__ float v[kTiles * 16 * kRow];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
   if ((int)blockIdx.x >= *a.tile_count) return;
   const AdapterTile tile = a.tiles[blockIdx.x];
@@ -315,116 +346,151 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(UpArgs a) {
   if (!with && a.skip_rows_without) return;
   const half_t *w = a.w + (int64_t)max(tile.adapter, 0) * a.rank * a.features;
   const float scaling = with ? a.scaling[tile.adapter] : 0.f;
+  const int64_t from = blockIdx.y * a.range, to = min(a.features, from + a.range), first = from + wave * 64;
+
+  half8_t wf[2][4][kChunks], y[kTiles][2];
+  int64_t row[kTiles];
+  const auto load_weights = [&](int set, int64_t n0) {
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const half_t *p = w + min(n0 + 16 * (m >> 2) + 4 * f + (m & 3), a.features - 1) * a.rank;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (c * 32 < a.rank) wf[set][f][c] = load8_any<kWide>(p, c * 32 + g * 8, a.rank);
+    }
+  };
+  const auto load_y = [&](int t, int64_t n0) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int64_t n = n0 + 16 * g + 8 * half;
+      y[t][half] = half8_t{};
+      if (a.y) y[t][half] = load8<kWide>(a.y + row[t] * a.y_stride + n, to - n);
+    }
+  };
+  if (with && first < to) load_weights(0, first);
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) row[t] = a.order[tile.begin + min(t * 16 + m, tile.count - 1)];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) load_y(t, first);
 
   half8_t hi[kTiles][kChunks], lo[kTiles][kChunks];
   float back[kTiles];
-  int64_t row[kTiles];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    const int i = min(t * 16 + m, tile.count - 1);
-    row[t] = a.order[tile.begin + i];
-    back[t] = 0.f;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) hi[t][c] = lo[t][c] = half8_t{};
-    if (!with) continue;
-    float v[kChunks][8], most = 0.f;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[c][j] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float *from = a.v + ((int64_t)s * a.rows + tile.begin + i) * kRank;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const float4_t u0 = *(const float4_t *)(from + c * 32 + g * 8), u1 = *(const float4_t *)(from + c * 32 + g * 8 + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[c][j] += u0[j], v[c][4 + j] += u1[j];
-      }
+  if (with) {
+    for (int n = threadIdx.x; n < tile.count * (kRank / 4); n += kThreads) {
+      const int i = n / (kRank / 4), r = n % (kRank / 4) * 4;
+      *(float4_t *)(v + i * kRow + r) = sum_of_splits(a.v + (int64_t)(tile.begin + i) * kRank + r, a.rows * kRank, a.splits);
     }
+    __syncthreads();
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+    for (int t = 0; t < kTiles; ++t) {
+      const float *p = v + min(t * 16 + m, tile.count - 1) * kRow + g * 8;
+      float most = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[c][j]));
-    most = fmaxf(most, __shfl_xor(most, 16));
-    most = fmaxf(most, __shfl_xor(most, 32));
-    const float power = normal_power(most, back[t]);
-    back[t] *= scaling;
+      for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(p[c * 32 + j]));
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const float power = normal_power(most, back[t]);
+      back[t] *= scaling;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        half_t h, l;
-        split_of(v[c][j] * power, h, l);
-        hi[t][c][j] = h, lo[t][c][j] = l;
-      }
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          half_t h, l;
+          split_of(p[c * 32 + j] * power, h, l);
+          hi[t][c][j] = h, lo[t][c][j] = l;
+        }
+    }
   }
 
-  half_t *turned = (half_t *)shared + wave * 64 * kRow;
-  const int64_t from = blockIdx.y * a.range, to = min(a.features, from + a.range);
-  for (int64_t n0 = from + wave * 64; n0 < to; n0 += kWaves * 64) {
-    float4_t acc[kTiles][4];
+  const auto piece = [&](int set, int64_t n0) {
+    const int64_t next = n0 + kWaves * 64;
+    if (with && next < to) load_weights(set ^ 1, next);
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
+    for (int t = 0; t < kTiles; ++t) {
+      float4_t acc[4];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) acc[t][f] = float4_t{};
-    if (with) {
-      if (kTurned) {
-        // [rank][64 features] to [features][rank], two ranks at a time; ranks behind the last are zeros
-        for (int n = lane; n < kRank / 2 * 8; n += 64) {
-          const int c = n % 8, r = n / 8 * 2;
-          const half_t *p = w + r * a.features + n0 + c * 8;
-          const int64_t left = to - n0 - c * 8;
-          const half8_t u0 = load8<kWide>(p, r < a.rank ? left : 0), u1 = load8<kWide>(p + a.features, r + 1 < a.rank ? left : 0);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) *(uint32_t *)(turned + (c * 8 + j) * kRow + r) = pair_of(u0[j], u1[j]);
-        }
-        wave_lds_fence();
-      }
-#pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        const int feature = 16 * (m >> 2) + 4 * f + (m & 3);
+      for (int f = 0; f < 4; ++f) acc[f] = float4_t{};
+      if (with) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           if (c * 32 >= a.rank) continue;
-          half8_t wf;
-          if (kTurned) {
-            wf = *(const half8_t *)(turned + feature * kRow + c * 32 + g * 8);
-          } else {
-            const int64_t n = min(n0 + feature, a.features - 1);
-            wf = load8<kWide>(w + n * a.rank + c * 32 + g * 8, a.rank - (c * 32 + g * 8));
-          }
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            acc[t][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, hi[t][c], acc[t][f], 0, 0, 0);
-            acc[t][f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, lo[t][c], acc[t][f], 0, 0, 0);
-          }
+          for (int f = 0; f < 4; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[set][f][c], hi[t][c], acc[f], 0, 0, 0);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[set][f][c], lo[t][c], acc[f], 0, 0, 0);
         }
-      }
-      if (kTurned) wave_lds_fence();
-    }
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      if (t * 16 + m >= tile.count) continue;
+        for (int f = 0; f < 4; ++f) acc[f] *= back[t];
+      }
+      const bool there = t * 16 + m < tile.count;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int64_t n = n0 + 16 * g + 8 * half;
-        if (n >= to) continue;
-        half8_t y = {};
-        if (a.y) y = load8<kWide>(a.y + row[t] * a.y_stride + n, to - n);
+        half8_t r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          // (tile f, row 4 g + i of the accumulators is feature 16 g + 4 f + i)
-          const float sum = (float)y[j] + acc[t][2 * half + j / 4][j % 4] * back[t];
-          y[j] = (half_t)apply_activation(sum, a.act);
-        }
+        for (int j = 0; j < 8; ++j)  // (tile f, row 4 g + i of the accumulators is feature 16 g + 4 f + i)
+          r[j] = (half_t)apply_activation((float)y[t][half][j] + acc[2 * half + j / 4][j % 4], a.act);
         half_t *o = a.out + row[t] * a.out_stride + n;
         if (kWide) {
-          *(half8_t *)o = y;
+          if (there && n < to) *(half8_t *)o = r;
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (n + j < to) o[j] = y[j];
+            if (there && n + j < to) o[j] = r[j];
         }
+      }
+      if (next < to) load_y(t, next);
+    }
+  };
+  for (int64_t n0 = first; n0 < to; n0 += 2 * kWaves * 64) {
+    piece(0, n0);
+    if (n0 + kWaves * 64 < to) piece(1, n0 + kWaves * 64);
+  }
+}
+
+// The gradients contract the other axis of each weight: both are turned first, [rows][columns] to [columns][rows] for every
+// adapter that has rows (a gradient of 4 bytes an element is written for every one of them, so this never dominates).
+struct TurnArgs {
+  const half_t *from[2];
+  half_t *to[2];
+  int64_t rows[2], columns[2];
+  const int *parts_of;
+  bool wide;  // rows and columns of both are multiples of 8, 16-byte aligned
+};
+
+__global__ __launch_bounds__(kThreads) void adapter_turn_kernel(TurnArgs a) {
+  __shared__ half_t piece[64][72];
+  const int which = blockIdx.z, adapter = blockIdx.y, tid = threadIdx.x;
+  if (a.parts_of[2 * adapter + 1] == 0) return;
+  const int64_t rows = which ? a.rows[1] : a.rows[0], columns = which ? a.columns[1] : a.columns[0];
+  const int64_t across = (columns + 63) / 64, pieces = (rows + 63) / 64 * across;
+  const half_t *from = (which ? a.from[1] : a.from[0]) + adapter * rows * columns;
+  half_t *to = (which ? a.to[1] : a.to[0]) + adapter * rows * columns;
+  for (int64_t n = blockIdx.x; n < pieces; n += gridDim.x) {
+    const int64_t r0 = n / across * 64, c0 = n % across * 64;
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < 64 * 8; i += kThreads) {
+      const int64_t r = r0 + i / 8, c = c0 + i % 8 * 8;
+      if (r >= rows) continue;
+      *(half8_t *)&piece[i / 8][i % 8 * 8] = a.wide ? load8<true>(from + r * columns + c, columns - c) : load8<false>(from + r * columns + c, columns - c);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < 64 * 8; i += kThreads) {
+      const int64_t c = c0 + i / 8, r = r0 + i % 8 * 8;
+      if (c >= columns) continue;
+      half8_t v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = piece[i % 8 * 8 + j][i / 8];
+      if (a.wide) {
+        if (r < rows) *(half8_t *)(to + c * rows + r) = v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (r + j < rows) to[c * rows + r + j] = v[j];
       }
     }
   }
@@ -433,12 +499,13 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(UpArgs a) {
 struct OuterSide {
   const half_t *x;  // [rows][features]
   int64_t x_stride, features;
-  const float *v;  // [splits][rows][kRank]
+  const float *v;     // [splits][rows][kRank]
+  const float *most;  // [splits][tiles]
   int splits;
-  half_t *operand;  // [segments][hi, lo][kRank][512]
+  half_t *operand;  // [segments][hi, lo][kRank][kAdapterSegment]
   float *back;      // [segments]
   float *grad;      // [adapters][rank][features], turned: [adapters][features][rank]
-  float *parts;     // [parts][rank][features]
+  float *parts;     // [parts], the same
   bool turned;
 };
 
@@ -448,56 +515,71 @@ struct OuterArgs {
   const int *segment_count, *order, *parts_of;
   const float *scaling;
   int64_t rows;
-  int rank, adapters;
+  int rank, adapters, most_tiles;
+  bool large;
 };
 
-// v of a segment as the other product's operand: summed over the splits, scaled by a power of two, split, transposed
+// v of a segment as the other product's operand: 64 rows a workgroup, summed over the splits, scaled by the segment's power of
+// two, split, transposed.  The power comes from the largest part times the number of splits, which is no less than the
+// largest sum; what it is too large by costs that many of the 22 bits.
 template <int kRank>
 __global__ __launch_bounds__(kThreads) void adapter_operand_kernel(OuterArgs a) {
-  __shared__ float wave_most[kWaves];
-  const OuterSide &side = a.side[blockIdx.y];
+  constexpr int kRow = 64 + 8;
+  __shared__ half_t piece[2][kRank][kRow];
+  const OuterSide &side = blockIdx.z ? a.side[1] : a.side[0];
   if ((int)blockIdx.x >= *a.segment_count) return;
   const AdapterTile seg = a.segments[blockIdx.x];
-  const int tid = threadIdx.x;
-  half_t *hi = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment, *lo = hi + kRank * kAdapterSegment;
-  const auto value = [&](int i, int r) {
-    float sum = 0.f;
-    for (int s = 0; s < side.splits; ++s) sum += side.v[((int64_t)s * a.rows + seg.begin + i) * kRank + r];
-    return sum;
-  };
+  const int i0 = blockIdx.y * 64, tid = threadIdx.x, lane = tid & 63;
+  if (i0 >= seg.count) return;
+  const int per_tile = a.large ? kAdapterLargeTile : kAdapterSmallTile, tiles = (seg.count + per_tile - 1) / per_tile;
+  const float *most_of = side.most + (a.large ? seg.first_large : seg.first);
   float most = 0.f;
-  for (int n = tid; n < seg.count * kRank; n += kThreads) most = fmaxf(most, fabsf(value(n / kRank, n % kRank)));
+  for (int n = lane; n < tiles * side.splits; n += 64) most = fmaxf(most, most_of[(int64_t)(n / tiles) * a.most_tiles + n % tiles]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  if ((tid & 63) == 0) wave_most[tid >> 6] = most;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_most[w]);
+  most *= side.splits;
   float back;
   const float power = normal_power(most, back);
-  if (tid == 0) side.back[blockIdx.x] = back * a.scaling[seg.adapter];
-  for (int n = tid; n < kAdapterSegment * kRank; n += kThreads) {
-    const int i = n / kRank, r = n % kRank;
-    half_t h = (half_t)0.f, l = (half_t)0.f;
-    if (i < seg.count) split_of(value(i, r) * power, h, l);
-    hi[r * kAdapterSegment + i] = h, lo[r * kAdapterSegment + i] = l;
+  if (i0 == 0 && tid == 0) side.back[blockIdx.x] = back * a.scaling[seg.adapter];
+  for (int n = tid; n < 64 * kRank / 4; n += kThreads) {
+    const int i = n / (kRank / 4), r = n % (kRank / 4) * 4;
+    float4_t sum = {};
+    if (i0 + i < seg.count) sum = sum_of_splits(side.v + (int64_t)(seg.begin + i0 + i) * kRank + r, a.rows * kRank, side.splits);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      half_t h, l;
+      split_of(sum[j] * power, h, l);
+      piece[0][r + j][i] = h, piece[1][r + j][i] = l;
+    }
+  }
+  __syncthreads();
+  half_t *to = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment;
+  for (int n = tid; n < 2 * kRank * 8; n += kThreads) {
+    const int which = n / (kRank * 8), r = n / 8 % kRank, i = n % 8 * 8;
+    *(half8_t *)(to + (int64_t)(which * kRank + r) * kAdapterSegment + i0 + i) = *(const half8_t *)&piece[which][r][i];
   }
 }
 
 // 128 features of one segment's product; the four waves take every fourth 32 rows and meet in LDS.  The rows are loaded as
 // they lie (8 features a lane, 8 rows) and paired in registers: operand c has feature 8 m + c, so that a lane ends with 8
-// consecutive features of 4 ranks.
+// consecutive features of 4 ranks.  Rows are loaded two steps ahead, the operand one: one wave a SIMD with 512 registers keeps
+// more bytes on their way than two with 256 (whose steps waited for the operand).
 template <int kRank, bool kWide>
-__global__ __launch_bounds__(kThreads) void adapter_outer_kernel(OuterArgs a) {
+__global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a) {
   constexpr int kRankTiles = kRank / 16 < 4 ? kRank / 16 : 4;  // 64 ranks at most at a time: blockIdx.z
-  __shared__ float shared[16 * (128 + 4) * kWaves];
+  constexpr int kRow = 128 + 4;
+  __shared__ float shared[kWaves * 16 * kRow];  // at first the segment's rows
+  int *order = (int *)shared;
+  static_assert(sizeof(shared) >= kAdapterSegment * sizeof(int), "a segment's rows fit");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
   const bool second = blockIdx.z & 1;
   const int rank0 = (blockIdx.z >> 1) * 64;
   const OuterSide &side = second ? a.side[1] : a.side[0];
-  if ((int)blockIdx.x >= *a.segment_count || (int64_t)blockIdx.y * 128 >= side.features) return;
+  if ((int)blockIdx.x >= *a.segment_count || (int64_t)blockIdx.y * 128 >= side.features || rank0 >= a.rank) return;
   const AdapterTile seg = a.segments[blockIdx.x];
-  const half_t *hi = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment, *lo = hi + kRank * kAdapterSegment;
+  for (int n = threadIdx.x; n < seg.count; n += kThreads) order[n] = a.order[seg.begin + n];
+  __syncthreads();
+  const half_t *hi = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment;
   const int64_t f = (int64_t)blockIdx.y * 128 + m * 8;
 
   float4_t acc[kRankTiles][8];
@@ -505,53 +587,73 @@ __global__ __launch_bounds__(kThreads) void adapter_outer_kernel(OuterArgs a) {
   for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
     for (int c = 0; c < 8; ++c) acc[r][c] = float4_t{};
-  for (int i0 = wave * 32; i0 < seg.count; i0 += kWaves * 32) {
-    half8_t x[8];
+  half8_t x[2][8], h[2][kRankTiles], l[2][kRankTiles];
+  const auto load = [&](int set, int i0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int i = i0 + g * 8 + j;
-      x[j] = half8_t{};
-      if (i < seg.count) x[j] = load8<kWide>(side.x + (int64_t)a.order[seg.begin + i] * side.x_stride + f, side.features - f);
+      // (rows behind the last have zeros in the other operand; features behind the last are not stored)
+      const int i = min(i0 + g * 8 + j, seg.count - 1);
+      x[set][j] = load8_any<kWide>(side.x + (int64_t)order[i] * side.x_stride, f, side.features);
     }
+  };
+  const auto load_operand = [&](int set, int i0) {
+    const half_t *at = hi + (int64_t)(rank0 + m) * kAdapterSegment + i0 + g * 8;
+#pragma unroll
+    for (int r = 0; r < kRankTiles; ++r) {
+      h[set][r] = *(const half8_t *)(at + r * 16 * kAdapterSegment);
+      l[set][r] = *(const half8_t *)(at + (kRank + r * 16) * kAdapterSegment);
+    }
+  };
+  constexpr int kStep = kWaves * 32;
+  const auto multiply = [&](int set, int i0) {
     half8_t xf[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) xf[c][j] = x[j][c];
+      for (int j = 0; j < 8; ++j) xf[c][j] = x[set][j][c];
+    // (the operand first: loads arrive in order, and it is needed a step before these rows)
+    if (i0 + kStep < seg.count) load_operand(set ^ 1, i0 + kStep);
+    if (i0 + 2 * kStep < seg.count) load(set, i0 + 2 * kStep);
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) {
       if (rank0 + r * 16 >= a.rank) continue;
-      const int64_t at = (int64_t)(rank0 + r * 16 + m) * kAdapterSegment + i0 + g * 8;
-      const half8_t h = *(const half8_t *)(hi + at), l = *(const half8_t *)(lo + at);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, xf[c], acc[r][c], 0, 0, 0);
-        acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, xf[c], acc[r][c], 0, 0, 0);
-      }
+      for (int c = 0; c < 8; ++c) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[set][r], xf[c], acc[r][c], 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[set][r], xf[c], acc[r][c], 0, 0, 0);
     }
+  };
+  const int start = wave * 32;
+  if (start < seg.count) load(0, start), load_operand(0, start);
+  if (start + kStep < seg.count) load(1, start + kStep);
+  for (int i0 = start; i0 < seg.count; i0 += 2 * kStep) {
+    multiply(0, i0);
+    if (i0 + kStep < seg.count) multiply(1, i0 + kStep);
   }
   const float back = side.back[blockIdx.x];
-  const bool direct = seg.part < 0;
-  float *out = direct ? side.grad + (int64_t)seg.adapter * a.rank * side.features : side.parts + (int64_t)seg.part * a.rank * side.features;
+  const int64_t f0 = (int64_t)blockIdx.y * 128;
+  float *out = seg.part < 0 ? side.grad + (int64_t)seg.adapter * a.rank * side.features : side.parts + (int64_t)seg.part * a.rank * side.features;
 #pragma unroll
   for (int r = 0; r < kRankTiles; ++r) {
     if (rank0 + r * 16 >= a.rank) continue;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < 8; ++c) shared[(wave * 16 + 4 * g + i) * 132 + m * 8 + c] = acc[r][c][i];
+    for (int i = 0; i < 4; ++i) {
+      float *to = shared + (wave * 16 + 4 * g + i) * kRow + m * 8;
+      *(float4_t *)to = float4_t{acc[r][0][i], acc[r][1][i], acc[r][2][i], acc[r][3][i]};
+      *(float4_t *)(to + 4) = float4_t{acc[r][4][i], acc[r][5][i], acc[r][6][i], acc[r][7][i]};
+    }
     __syncthreads();
     for (int n = threadIdx.x; n < 16 * 128; n += kThreads) {
-      // (a gradient [features][rank] is written rank by rank)
-      const int rr = direct && side.turned ? n % 16 : n / 128, ff = direct && side.turned ? n / 16 : n % 128;
+      // (a gradient [features][rank] is written 16 ranks of a feature at a time)
+      const int rr = side.turned ? n % 16 : n / 128, ff = side.turned ? n / 16 : n % 128;
       const int rank = rank0 + r * 16 + rr;
-      const int64_t feature = (int64_t)blockIdx.y * 128 + ff;
+      const int64_t feature = f0 + ff;
       if (rank >= a.rank || feature >= side.features) continue;
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) sum += shared[(w * 16 + rr) * 132 + ff];
-      out[direct && side.turned ? feature * a.rank + rank : rank * side.features + feature] = sum * back;
+      for (int w = 0; w < kWaves; ++w) sum += shared[(w * 16 + rr) * kRow + ff];
+      out[side.turned ? feature * a.rank + rank : rank * side.features + feature] = sum * back;
     }
   }
 }
@@ -563,10 +665,10 @@ __global__ __launch_bounds__(kThreads) void adapter_sum_kernel(OuterArgs a) {
   if (segments == 1) return;
   const int64_t size = a.rank * side.features;
   float *grad = side.grad + adapter * size;
+  const float *parts = side.parts + first * size;
   for (int64_t n = (int64_t)blockIdx.x * kThreads + threadIdx.x; n < size; n += (int64_t)gridDim.x * kThreads) {
-    const int64_t at = side.turned ? n % a.rank * side.features + n / a.rank : n;
     float sum = 0.f;
-    for (int s = 0; s < segments; ++s) sum += side.parts[(first + s) * size + at];
+    for (int s = 0; s < segments; ++s) sum += parts[s * size + n];
     grad[n] = sum;
   }
 }
@@ -578,7 +680,7 @@ int rank_class(int64_t rank) { return rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 // Workgroups that fill the device twice over where the features allow it, each with at least 512 features (128 a wave)
 int64_t down_splits(int64_t tiles, int64_t features) {
-  const int64_t most = (features + kWaves * kStep - 1) / (kWaves * kStep), want = (512 + tiles - 1) / tiles;
+  const int64_t most = (features + 511) / 512, want = (512 + tiles - 1) / tiles;
   return want < most ? want : most > 0 ? most : 1;
 }
 
@@ -601,48 +703,42 @@ int allow_lds(const void *kernel, size_t bytes, const char *who) {
   return e == hipSuccess ? GQ_OK : fail((int)e, "%s: %s", who, hipGetErrorString(e));
 }
 
-template <int kRank, int kTiles, bool kWide, bool kTurned>
+template <int kRank, int kTiles, bool kWide>
 int start_down(const DownArgs &a, int64_t tiles, int64_t splits, hipStream_t stream) {
-  const size_t sums = (size_t)kWaves * 16 * (kRank + 4) * sizeof(float);
-  const size_t turned = kTurned ? (size_t)kWaves * kRank * kTurnedRow * sizeof(half_t) : 0;
-  const size_t lds = sums > turned ? sums : turned;
-  if (int rc = allow_lds((const void *)adapter_down_kernel<kRank, kTiles, kWide, kTurned>, lds, "adapter_down_kernel")) return rc;
-  adapter_down_kernel<kRank, kTiles, kWide, kTurned><<<dim3((unsigned)tiles, (unsigned)splits), kThreads, lds, stream>>>(a);
+  const size_t lds = (size_t)kWaves * 16 * (kRank + 4) * sizeof(float);
+  adapter_down_kernel<kRank, kTiles, kWide><<<dim3((unsigned)tiles, (unsigned)splits), kThreads, lds, stream>>>(a);
   return check_launch("adapter_down_kernel");
 }
 
-template <int kRank, int kTiles, bool kWide, bool kTurned>
+template <int kRank, int kTiles, bool kWide>
 int start_up(const UpArgs &a, int64_t tiles, int64_t ranges, hipStream_t stream) {
-  const size_t lds = kTurned ? (size_t)kWaves * 64 * (kRank + 8) * sizeof(half_t) : 0;
-  if (int rc = allow_lds((const void *)adapter_up_kernel<kRank, kTiles, kWide, kTurned>, lds, "adapter_up_kernel")) return rc;
-  adapter_up_kernel<kRank, kTiles, kWide, kTurned><<<dim3((unsigned)tiles, (unsigned)ranges), kThreads, lds, stream>>>(a);
+  adapter_up_kernel<kRank, kTiles, kWide><<<dim3((unsigned)tiles, (unsigned)ranges), kThreads, 0, stream>>>(a);
   return check_launch("adapter_up_kernel");
 }
 
-#define GQ_BY_SHAPE(START, TURNED, ...)                                                                                   \
-  (kRankClass == 32    ? (large ? (wide ? START<32, 4, true, TURNED>(__VA_ARGS__) : START<32, 4, false, TURNED>(__VA_ARGS__))    \
-                                : (wide ? START<32, 1, true, TURNED>(__VA_ARGS__) : START<32, 1, false, TURNED>(__VA_ARGS__)))   \
-   : kRankClass == 64  ? (large ? (wide ? START<64, 4, true, TURNED>(__VA_ARGS__) : START<64, 4, false, TURNED>(__VA_ARGS__))    \
-                                : (wide ? START<64, 1, true, TURNED>(__VA_ARGS__) : START<64, 1, false, TURNED>(__VA_ARGS__)))   \
-                       : (large ? (wide ? START<128, 4, true, TURNED>(__VA_ARGS__) : START<128, 4, false, TURNED>(__VA_ARGS__))  \
-                                : (wide ? START<128, 1, true, TURNED>(__VA_ARGS__) : START<128, 1, false, TURNED>(__VA_ARGS__))))
+#define GQ_BY_SHAPE(START, ...)                                                                                 \
+  (kRankClass == 32    ? (large ? (wide ? START<32, 4, true>(__VA_ARGS__) : START<32, 4, false>(__VA_ARGS__))    \
+                                : (wide ? START<32, 1, true>(__VA_ARGS__) : START<32, 1, false>(__VA_ARGS__)))   \
+   : kRankClass == 64  ? (large ? (wide ? START<64, 4, true>(__VA_ARGS__) : START<64, 4, false>(__VA_ARGS__))    \
+                                : (wide ? START<64, 1, true>(__VA_ARGS__) : START<64, 1, false>(__VA_ARGS__)))   \
+                       : (large ? (wide ? START<128, 4, true>(__VA_ARGS__) : START<128, 4, false>(__VA_ARGS__))  \
+                                : (wide ? START<128, 1, true>(__VA_ARGS__) : START<128, 1, false>(__VA_ARGS__))))
 
 bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
-int launch_down(const Batch &b, const half_t *x, int64_t x_stride, const half_t *w, bool turned, int64_t features, int64_t rank,
-                float *v, int64_t splits, hipStream_t stream) {
+int launch_down(const Batch &b, const half_t *x, int64_t x_stride, const half_t *w, int64_t features, int64_t rank, float *v, float *most,
+                int64_t splits, hipStream_t stream) {
   DownArgs a;
   a.x = x, a.w = w, a.x_stride = x_stride, a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0);
-  a.order = b.words + b.plan.order, a.v = v, a.rows = b.plan.rows, a.features = features, a.rank = (int)rank;
-  a.split = round_up((features + splits - 1) / splits, kWaves * kStep);
-  const bool large = b.large, wide = aligned16(x) && aligned16(w) && x_stride % 8 == 0 && features % 8 == 0 && (!turned || rank % 8 == 0);
+  a.order = b.words + b.plan.order, a.v = v, a.most = most, a.rows = b.plan.rows, a.features = features, a.rank = (int)rank;
+  a.split = round_up((features + splits - 1) / splits, 128), a.most_tiles = (int)b.most_tiles();
+  const bool large = b.large, wide = aligned16(x) && aligned16(w) && x_stride % 8 == 0 && features % 8 == 0;
   const int kRankClass = rank_class(rank);
-  return turned ? GQ_BY_SHAPE(start_down, true, a, b.most_tiles(), splits, stream)
-                : GQ_BY_SHAPE(start_down, false, a, b.most_tiles(), splits, stream);
+  return GQ_BY_SHAPE(start_down, a, b.most_tiles(), splits, stream);
 }
 
-int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, bool turned, const float *scaling, const half_t *y,
-              int64_t y_stride, half_t *out, int64_t out_stride, int64_t features, int64_t rank, int act, hipStream_t stream) {
+int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, const float *scaling, const half_t *y, int64_t y_stride,
+              half_t *out, int64_t out_stride, int64_t features, int64_t rank, int act, hipStream_t stream) {
   UpArgs a;
   a.v = v, a.w = w, a.scaling = scaling, a.y = y, a.out = out, a.y_stride = y_stride, a.out_stride = out_stride;
   a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0), a.order = b.words + b.plan.order;
@@ -651,17 +747,17 @@ int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, b
   const int64_t tiles = b.most_tiles(), most = (features + 255) / 256, want = (1024 + tiles - 1) / tiles;
   a.range = round_up((features + (want < most ? want : most) - 1) / (want < most ? want : most), 256);
   const int64_t ranges = (features + a.range - 1) / a.range;
-  const bool large = b.large;
-  const bool wide = aligned16(y) && aligned16(out) && aligned16(w) && y_stride % 8 == 0 && out_stride % 8 == 0 && features % 8 == 0 &&
-                    (turned || rank % 8 == 0);
+  const bool large = b.large, wide = aligned16(y) && aligned16(out) && aligned16(w) && y_stride % 8 == 0 && out_stride % 8 == 0 &&
+                                     features % 8 == 0 && rank % 8 == 0;
   const int kRankClass = rank_class(rank);
-  return turned ? GQ_BY_SHAPE(start_up, true, a, tiles, ranges, stream) : GQ_BY_SHAPE(start_up, false, a, tiles, ranges, stream);
+  return GQ_BY_SHAPE(start_up, a, tiles, ranges, stream);
 }
 
 template <int kRank>
 int launch_outer(const OuterArgs &a, const PlanLayout &plan, bool wide, hipStream_t stream) {
   const int64_t features = a.side[0].features > a.side[1].features ? a.side[0].features : a.side[1].features;
-  adapter_operand_kernel<kRank><<<dim3((unsigned)plan.most_segments, 2), kThreads, 0, stream>>>(a);
+  const int64_t longest = plan.rows < kAdapterSegment ? plan.rows : kAdapterSegment;
+  adapter_operand_kernel<kRank><<<dim3((unsigned)plan.most_segments, (unsigned)((longest + 63) / 64), 2), kThreads, 0, stream>>>(a);
   int rc = check_launch("adapter_operand_kernel");
   if (rc != GQ_OK) return rc;
   const dim3 grid((unsigned)plan.most_segments, (unsigned)((features + 127) / 128), 2 * (kRank > 64 ? 2 : 1));
@@ -672,13 +768,13 @@ int launch_outer(const OuterArgs &a, const PlanLayout &plan, bool wide, hipStrea
   rc = check_launch("adapter_outer_kernel");
   if (rc != GQ_OK) return rc;
   const int64_t each = (a.rank * features + kThreads - 1) / kThreads;
-  adapter_sum_kernel<<<dim3((unsigned)(each < 512 ? each : 512), (unsigned)a.adapters, 2), kThreads, 0, stream>>>(a);
+  adapter_sum_kernel<<<dim3((unsigned)(each < 1024 ? each : 1024), (unsigned)a.adapters, 2), kThreads, 0, stream>>>(a);
   return check_launch("adapter_sum_kernel");
 }
 
 struct GradLayout {
-  int64_t v, dv, operand[2], back[2], parts[2], bytes;
-  GradLayout(const PlanLayout &plan, int64_t in, int64_t out, int64_t rank, int64_t in_splits, int64_t out_splits) {
+  int64_t v, dv, most[2], turned[2], operand[2], back[2], parts[2], bytes;
+  GradLayout(const PlanLayout &plan, int64_t most_tiles, int64_t in, int64_t out, int64_t rank, int64_t in_splits, int64_t out_splits) {
     const int64_t width = rank_class(rank);
     int64_t at = 0;
     const auto take = [&](int64_t n) {
@@ -688,6 +784,8 @@ struct GradLayout {
     };
     v = take(in_splits * plan.rows * width * 4), dv = take(out_splits * plan.rows * width * 4);
     for (int i = 0; i < 2; ++i) {
+      most[i] = take((i ? out_splits : in_splits) * most_tiles * 4);
+      turned[i] = take(plan.adapters * rank * (i ? out : in) * 2);
       operand[i] = take(plan.most_segments * 2 * width * kAdapterSegment * 2), back[i] = take(plan.most_segments * 4);
       parts[i] = take(plan.most_parts * rank * (i ? out : in) * 4);
     }
@@ -719,44 +817,54 @@ int launch_adapter_apply(const gq_adapters &w, const void *plan, int64_t rows, c
                          int64_t y_stride, uint16_t *out, int64_t out_stride, int act, void *workspace, hipStream_t stream) {
   const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows)};
   const int64_t splits = down_splits(b.most_tiles(), w.in_features);
-  const int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, false, w.in_features, w.rank, (float *)workspace, splits, stream);
+  const int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, w.in_features, w.rank, (float *)workspace, nullptr, splits, stream);
   if (rc != GQ_OK) return rc;
-  return launch_up(b, (const float *)workspace, splits, (const half_t *)w.up, false, w.scaling, (const half_t *)y, y_stride, (half_t *)out,
-                   out_stride, w.out_features, w.rank, act, stream);
+  return launch_up(b, (const float *)workspace, splits, (const half_t *)w.up, w.scaling, (const half_t *)y, y_stride, (half_t *)out, out_stride,
+                   w.out_features, w.rank, act, stream);
 }
 
 int64_t adapter_grad_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t out, int64_t rank) {
   const PlanLayout plan(rows, adapters);
-  return GradLayout(plan, in, out, rank, down_splits(tiles_at_most(plan), in), down_splits(tiles_at_most(plan), out)).bytes;
+  const int64_t tiles = tiles_at_most(plan);
+  return GradLayout(plan, tiles, in, out, rank, down_splits(tiles, in), down_splits(tiles, out)).bytes;
 }
 
 int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, const uint16_t *x, int64_t x_stride, const uint16_t *dy,
                         int64_t dy_stride, const uint16_t *dx, int64_t dx_stride, uint16_t *dx_out, int64_t dx_out_stride, float *d_down,
                         float *d_up, void *workspace, hipStream_t stream) {
   const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows)};
-  const int64_t in_splits = down_splits(b.most_tiles(), w.in_features), out_splits = down_splits(b.most_tiles(), w.out_features);
-  const GradLayout l(b.plan, w.in_features, w.out_features, w.rank, in_splits, out_splits);
+  const int64_t in = w.in_features, out = w.out_features, tiles = b.most_tiles();
+  const int64_t in_splits = down_splits(tiles, in), out_splits = down_splits(tiles, out);
+  const GradLayout l(b.plan, tiles, in, out, w.rank, in_splits, out_splits);
   char *ws = (char *)workspace;
-  int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, false, w.in_features, w.rank, (float *)(ws + l.v), in_splits, stream);
+  half_t *down_turned = (half_t *)(ws + l.turned[0]), *up_turned = (half_t *)(ws + l.turned[1]);
+  const TurnArgs turn = {{(const half_t *)w.down, (const half_t *)w.up}, {down_turned, up_turned}, {w.rank, out}, {in, w.rank},
+                         b.words + b.plan.parts, (w.rank | in | out) % 8 == 0 && aligned16(w.down) && aligned16(w.up)};
+  const int64_t pieces = ((in > out ? in : out) + 63) / 64 * ((w.rank + 63) / 64);
+  adapter_turn_kernel<<<dim3((unsigned)(pieces < 512 ? pieces : 512), (unsigned)w.n_adapters, 2), kThreads, 0, stream>>>(turn);
+  int rc = check_launch("adapter_turn_kernel");
   if (rc == GQ_OK)
-    rc = launch_down(b, (const half_t *)dy, dy_stride, (const half_t *)w.up, true, w.out_features, w.rank, (float *)(ws + l.dv), out_splits, stream);
+    rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, in, w.rank, (float *)(ws + l.v), (float *)(ws + l.most[0]), in_splits, stream);
   if (rc == GQ_OK)
-    rc = launch_up(b, (const float *)(ws + l.dv), out_splits, (const half_t *)w.down, true, w.scaling, (const half_t *)dx, dx_stride,
-                   (half_t *)dx_out, dx_out_stride, w.in_features, w.rank, GQ_ACT_NONE, stream);
+    rc = launch_down(b, (const half_t *)dy, dy_stride, up_turned, out, w.rank, (float *)(ws + l.dv), (float *)(ws + l.most[1]), out_splits, stream);
+  if (rc == GQ_OK)
+    rc = launch_up(b, (const float *)(ws + l.dv), out_splits, down_turned, w.scaling, (const half_t *)dx, dx_stride, (half_t *)dx_out, dx_out_stride,
+                   in, w.rank, GQ_ACT_NONE, stream);
   if (rc != GQ_OK) return rc;
   OuterArgs a;
   // dA: the rows of x with dv;  dB: the rows of dy with v
   for (int i = 0; i < 2; ++i) {
     OuterSide &s = a.side[i];
-    s.x = (const half_t *)(i ? dy : x), s.x_stride = i ? dy_stride : x_stride, s.features = i ? w.out_features : w.in_features;
+    s.x = (const half_t *)(i ? dy : x), s.x_stride = i ? dy_stride : x_stride, s.features = i ? out : in;
     s.v = (const float *)(ws + (i ? l.v : l.dv)), s.splits = (int)(i ? in_splits : out_splits);
+    s.most = (const float *)(ws + l.most[i ? 0 : 1]);
     s.operand = (half_t *)(ws + l.operand[i]), s.back = (float *)(ws + l.back[i]), s.parts = (float *)(ws + l.parts[i]);
     s.grad = i ? d_up : d_down, s.turned = i == 1;
   }
   a.segments = (const AdapterTile *)(b.words + b.plan.segments), a.segment_count = b.words + b.plan.counts + 2;
   a.order = b.words + b.plan.order, a.parts_of = b.words + b.plan.parts, a.scaling = w.scaling;
-  a.rows = rows, a.rank = w.rank, a.adapters = (int)w.n_adapters;
-  const bool wide = aligned16(x) && aligned16(dy) && (x_stride | dy_stride | w.in_features | w.out_features) % 8 == 0;
+  a.rows = rows, a.rank = (int)w.rank, a.adapters = (int)w.n_adapters, a.most_tiles = (int)tiles, a.large = b.large;
+  const bool wide = aligned16(x) && aligned16(dy) && (x_stride | dy_stride | in | out) % 8 == 0;
   return rank_class(w.rank) == 32   ? launch_outer<32>(a, b.plan, wide, stream)
          : rank_class(w.rank) == 64 ? launch_outer<64>(a, b.plan, wide, stream)
                                     : launch_outer<128>(a, b.plan, wide, stream);
