@@ -316,6 +316,21 @@ __device__ __forceinline__ float normal_power(float most, float &back) {
   return ldexpf(1.f, -e);
 }
 
+// The epilogue on 8 values.  The tanh form of gelu is v s(2 u), s the logistic function: one exponential, where tanhf for
+// each of a lane's 64 values would make the kernel's code outgrow the instruction cache.
+__device__ __forceinline__ void activate(float (&v)[8], int act) {
+  if (act == GQ_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
+  } else if (act == GQ_ACT_GELU_TANH) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float u = 0.7978845608028654f * (v[j] + 0.044715f * (v[j] * v[j] * v[j]));
+      v[j] = v[j] / (1.f + __builtin_amdgcn_exp2f(-2.8853900817779268f * u));  // 2 log2(e)
+    }
+  }
+}
+
 // v summed over the splits, `p` a row's 4 ranks: four loads in flight
 __device__ __forceinline__ float4_t sum_of_splits(const float *p, int64_t stride, int splits) {
   float4_t sum = {};
@@ -429,9 +444,13 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
       for (int half = 0; half < 2; ++half) {
         const int64_t n = n0 + 16 * g + 8 * half;
         half8_t r;
+        float sum[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)  // (tile f, row 4 g + i of the accumulators is feature 16 g + 4 f + i)
-          r[j] = (half_t)apply_activation((float)y[t][half][j] + acc[2 * half + j / 4][j % 4], a.act);
+          sum[j] = (float)y[t][half][j] + acc[2 * half + j / 4][j % 4];
+        activate(sum, a.act);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = (half_t)sum[j];
         half_t *o = a.out + row[t] * a.out_stride + n;
         if (kWide) {
           if (there && n < to) *(half8_t *)o = r;

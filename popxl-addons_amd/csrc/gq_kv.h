@@ -39,30 +39,48 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatch &batch, int b) {
   return s;
 }
 
-// The sequence b and the index in it of unit `unit`, where sequence b has units(b) >= 0 of them: a wave's prefix sum over 64
-// sequences at a time.  Every lane gets the answer; false: there are fewer units.  `base` gets the units before b.
+// The sequence b that has unit `unit`, where sequence b has units(sequence) of them, and the units before b: a wave's prefix sum
+// over 64 sequences at a time.  Every lane gets the answer (uniform); false: there are fewer units.  (32 bits: the host sees
+// to it that there are fewer than 2^31.)
 template <typename F>
-__device__ __forceinline__ bool kv_locate(int64_t unit, int sequences, F units, int &b, int64_t &base) {
+__device__ __forceinline__ bool kv_locate(const KvBatch &batch, uint32_t unit, F units, int &b, KvSequence &s, uint32_t &base) {
   const int lane = threadIdx.x & 63;
   base = 0;
-  for (int b0 = 0; b0 < sequences; b0 += 64) {
-    const int64_t own = b0 + lane < sequences ? (int64_t)units(b0 + lane) : 0;
-    int64_t sum = own;
+  for (int b0 = 0; b0 < batch.sequences; b0 += 64) {
+    KvSequence own_s = {};
+    uint32_t own = 0;
+    if (b0 + lane < batch.sequences) {
+      own_s = kv_sequence(batch, b0 + lane);
+      own = units(own_s);
+    }
+    uint32_t sum = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t up = __shfl_up((long long)sum, d);
+      const uint32_t up = __shfl_up(sum, d);
       if (lane >= d) sum += up;
     }
-    const int64_t total = __shfl((long long)sum, 63);
+    const uint32_t total = __builtin_amdgcn_readlane(sum, 63);
     if (unit < base + total) {
       const int at = __builtin_ctzll(__ballot(base + sum > unit));
-      b = __builtin_amdgcn_readfirstlane(b0 + at);
-      base += __shfl((long long)(sum - own), at);
+      b = b0 + at;
+      s.begin = __builtin_amdgcn_readlane(own_s.begin, at), s.count = __builtin_amdgcn_readlane(own_s.count, at);
+      s.first = __builtin_amdgcn_readlane(own_s.first, at), s.length = __builtin_amdgcn_readlane(own_s.length, at);
+      base += __builtin_amdgcn_readlane(sum - own, at);
       return true;
     }
     base += total;
   }
   return false;
+}
+
+// Units of all sequences.
+template <typename F>
+__device__ __forceinline__ uint32_t kv_units(const KvBatch &batch, F units) {
+  uint32_t sum = 0;
+  for (int b = threadIdx.x & 63; b < batch.sequences; b += 64) sum += units(kv_sequence(batch, b));
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  return __builtin_amdgcn_readfirstlane(sum);
 }
 
 }  // namespace gq

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kRows = 16;
 constexpr int kMostGroups = 512;
+constexpr int kTileLeast = 64;
 
 struct AttentionArgs {
   KvCache cache;
@@ -44,29 +45,31 @@ struct Shape {  // one sequence's share of the work
 
 __device__ __forceinline__ Shape shape_of(const AttentionArgs &a, const KvSequence &s) {
   Shape r;
-  r.tiles = (int)(((int64_t)s.count * a.group + kRows - 1) / kRows);
+  r.tiles = (s.count * a.group + kRows - 1) / kRows;
   r.blocks = max(1, (s.length + kBlock - 1) / kBlock);
   return r;
 }
 
-__device__ __forceinline__ int64_t units_of(const AttentionArgs &a, int b) {
-  const Shape s = shape_of(a, kv_sequence(a.batch, b));
-  return (int64_t)s.tiles * s.blocks * a.cache.heads;
+__device__ __forceinline__ uint32_t units_of(const AttentionArgs &a, const KvSequence &s) {
+  const Shape shape = shape_of(a, s);
+  return (uint32_t)shape.tiles * shape.blocks * a.cache.heads;
 }
 
-__device__ __forceinline__ int64_t all_units(const AttentionArgs &a) {
-  int64_t sum = 0;
-  for (int b = threadIdx.x & 63; b < a.batch.sequences; b += 64) sum += units_of(a, b);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor((long long)sum, d);
-  return sum;
-}
-
-// Workgroups that take part: enough that each has four blocks, one for each wave.
-__device__ __forceinline__ int64_t active_groups(int64_t units, int groups) {
-  const int64_t want = (units + kWaves - 1) / kWaves;
-  return want < groups ? max(want, (int64_t)1) : groups;
-}
+// The cut of the units: `groups` workgroups take part, enough that each has four blocks, one for each wave; the first `more` of
+// them have one unit more than the others.
+struct Cut {
+  uint32_t units, groups, each, more;
+  __device__ Cut(uint32_t units_, uint32_t most) : units(units_) {
+    const uint32_t want = (units + kWaves - 1) / kWaves;
+    groups = min(max(want, 1u), most);
+    each = units / groups, more = units - each * groups;
+  }
+  __device__ uint32_t start(uint32_t group) const { return group * each + min(group, more); }
+  __device__ uint32_t owner(uint32_t unit) const {
+    const uint32_t large = more * (each + 1);
+    return unit < large ? unit / (each + 1) : more + (unit - large) / each;
+  }
+};
 
 __device__ __forceinline__ half2_t two_codes(uint32_t bytes, uint32_t selector) {
   const uint32_t w = __builtin_amdgcn_perm(0x64646464u, bytes, selector);
@@ -81,30 +84,64 @@ __device__ __forceinline__ half8_t eight_codes(uint32_t lo, uint32_t hi) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// DP: head_dim rounded up to 64, 128 or 256; dims behind head_dim are read as zeros of q and never stored.
+// 4 dims of a row of the result; a row that has seen nothing is zeros
+__device__ __forceinline__ void store_row(const AttentionArgs &a, const KvSequence &s, int h, int row, int d, float4_t value, float weight) {
+  const int token = row / a.group, member = row - token * a.group;
+  half_t *to = a.out + (s.begin + token) * a.o_token + (int64_t)(h * a.group + member) * a.o_head + d;
+  const float factor = weight == 0.f ? 0.f : 1.f / weight;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) to[j] = (half_t)(value[j] * factor);
+}
+
+// DP: head_dim rounded up to 64, 128 or 256; dims behind head_dim are read as zeros of q and never stored.  A block's values are
+// asked for before its scores are formed, the next block's keys before the probabilities: loads arrive in order, so that
+// each wait leaves the later ones on their way.
 template <int DP>
 __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(AttentionArgs a) {
   constexpr int kChunks = DP / 64, kTiles = DP / 16;
   extern __shared__ float shared[];  // [waves][kRows][DP + 4] and [waves][2][kRows]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int dim = a.cache.dim, heads = a.cache.heads;
-  const int64_t units = all_units(a), groups = active_groups(units, a.groups);
-  if (units == 0 || (int64_t)blockIdx.x >= groups) return;
-  int64_t unit = units * blockIdx.x / groups;
-  const int64_t end = units * (blockIdx.x + 1) / groups;
-  const int64_t start = unit;
+  const auto units_of_sequence = [&](const KvSequence &s) { return units_of(a, s); };
+  const Cut cut(kv_units(a.batch, units_of_sequence), a.groups);
+  if (blockIdx.x >= cut.groups) return;
+  const uint32_t start = cut.start(blockIdx.x), end = cut.start(blockIdx.x + 1);
+  uint32_t unit = start;
 
   while (unit < end) {
     int b;
-    int64_t base;
-    if (!kv_locate(unit, a.batch.sequences, [&](int i) { return units_of(a, i); }, b, base)) return;
-    const KvSequence s = kv_sequence(a.batch, b);
+    uint32_t base;
+    KvSequence s;
+    if (!kv_locate(a.batch, unit, units_of_sequence, b, s, base)) return;
     const Shape shape = shape_of(a, s);
-    const int64_t within = unit - base;
-    const int block0 = (int)(within % shape.blocks);
-    const int tile = (int)(within / shape.blocks % shape.tiles), h = (int)(within / shape.blocks / shape.tiles);
-    const int block1 = (int)min((int64_t)shape.blocks, block0 + end - unit);
+    const uint32_t which = (unit - base) / shape.blocks;
+    const int block0 = unit - base - which * shape.blocks, block1 = min((uint32_t)shape.blocks, block0 + end - unit);
+    const int h = which / shape.tiles, tile = which - h * shape.tiles;
     const int *table = a.batch.table + (int64_t)b * a.batch.width;
+    const int stop = min(block1, (s.length + kBlock - 1) / kBlock);  // (an empty sequence has no block to read)
+
+    // ids of blocks that are not there are -1
+    const auto id_of = [&](int block) {
+      const int id = block < stop ? __builtin_amdgcn_readfirstlane(table[block]) : -1;
+      return id < a.cache.n_blocks ? id : -1;
+    };
+    uint4_t kf[4][kChunks];
+    float key_scale = 0.f, value_scale = 0.f;
+    const auto load_keys = [&](int id) {
+      if (id < 0) return;
+      const int64_t place = (int64_t)id * heads + h;
+      const uint8_t *kc = a.cache.k_codes + place * kBlock * dim;
+      key_scale = a.cache.k_scale[place] * a.scale_log2, value_scale = a.cache.v_scale[place];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int key = 16 * (m >> 2) + 4 * t + (m & 3), d = min(c * 64 + g * 16, dim - 16);
+          kf[t][c] = *(const uint4_t *)(kc + key * dim + d);
+        }
+    };
+    int id = id_of(block0 + wave), next_id = id_of(block0 + wave + kWaves);
+    load_keys(id);
 
     // this lane's row of the tile: new token `token`, query head h * group + member
     const int row = tile * kRows + m, rows = s.count * a.group;
@@ -128,73 +165,67 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
     for (int i = 0; i < kTiles; ++i) o[i] = float4_t{};
     float most = -__builtin_inff(), sum = 0.f;
 
-    for (int block = block0 + wave; block < block1; block += kWaves) {
-      const int at = block * kBlock;
-      if (at >= s.length) continue;  // (the one block of an empty sequence: the table need not have a column for it)
-      const int id = __builtin_amdgcn_readfirstlane(table[block]);
-      if (id < 0 || id >= a.cache.n_blocks) continue;
-      const int64_t place = (int64_t)id * heads + h;
-      const uint8_t *kc = a.cache.k_codes + place * kBlock * dim, *vc = a.cache.v_codes + place * kBlock * dim;
-      const float ks = a.cache.k_scale[place] * a.scale_log2, vs = a.cache.v_scale[place];
-
-      uint4_t kf[4][kChunks];
+    for (int block = block0 + wave; block < stop; block += kWaves) {
+      const int at = block * kBlock, after = id_of(block + 2 * kWaves);
+      const float ks = key_scale, vs = value_scale;
+      if (id >= 0) {
+        const uint8_t *vc = a.cache.v_codes + ((int64_t)id * heads + h) * kBlock * dim;
+        uint4_t vf[kTiles];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int i = 0; i < kTiles; ++i) vf[i] = *(const uint4_t *)(vc + min(i * 16 + m, dim - 1) * kBlock + 16 * g);
+        float4_t score[4];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int key = 16 * (m >> 2) + 4 * t + (m & 3), d = min(c * 64 + g * 16, dim - 16);
-          kf[t][c] = *(const uint4_t *)(kc + key * dim + d);
+        for (int t = 0; t < 4; ++t) {
+          score[t] = float4_t{};
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(kf[t][c][0], kf[t][c][1]), qf[c][0], score[t], 0, 0, 0);
+            score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(kf[t][c][2], kf[t][c][3]), qf[c][1], score[t], 0, 0, 0);
+          }
         }
-      float4_t score[4];
+        load_keys(next_id);
+        const bool masked = at + kBlock - 1 > least;
+        float top = -__builtin_inff();
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        score[t] = float4_t{};
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(kf[t][c][0], kf[t][c][1]), qf[c][0], score[t], 0, 0, 0);
-          score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(kf[t][c][2], kf[t][c][3]), qf[c][1], score[t], 0, 0, 0);
+          for (int i = 0; i < 4; ++i) {
+            score[t][i] *= ks;
+            if (masked && at + 16 * g + 4 * t + i > position) score[t][i] = -__builtin_inff();
+            top = fmaxf(top, score[t][i]);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float next = fmaxf(most, top);
+        const float zero_point = next == -__builtin_inff() ? 0.f : next;  // (a row that has seen nothing: every p is 0)
+        const float keep = __builtin_amdgcn_exp2f(most - zero_point);
+        most = next;
+        half8_t pf[2];
+        float part = 0.f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(score[t][i] - zero_point);
+            part += p;
+            // (binary16 for the matrix product: at most 2^-11 of each p, the sum keeps all of it)
+            pf[t >> 1][4 * (t & 1) + i] = (half_t)p;
+          }
+        sum = sum * keep + part;
+        // a row that sees none of this block takes nothing from it, also where its scale is not finite
+        const float factor = at > position ? 0.f : vs;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          float4_t r = {};
+          r = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(vf[i][0], vf[i][1]), pf[0], r, 0, 0, 0);
+          r = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(vf[i][2], vf[i][3]), pf[1], r, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(r[j], factor, o[i][j] * keep);
         }
+      } else {
+        load_keys(next_id);
       }
-      const bool masked = at + kBlock - 1 > least;
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          score[t][i] *= ks;
-          if (masked && at + 16 * g + 4 * t + i > position) score[t][i] = -__builtin_inff();
-          top = fmaxf(top, score[t][i]);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float next = fmaxf(most, top);
-      const float zero_point = next == -__builtin_inff() ? 0.f : next;  // (a row that has seen nothing: every p is 0)
-      const float keep = __builtin_amdgcn_exp2f(most - zero_point);
-      most = next;
-      half8_t pf[2];
-      float part = 0.f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(score[t][i] - zero_point);
-          part += p;
-          // (binary16 for the matrix product: at most 2^-11 of each p, the sum keeps all of it)
-          pf[t >> 1][4 * (t & 1) + i] = (half_t)p;
-        }
-      sum = sum * keep + part;
-      // a row that sees none of this block takes nothing from it, also where its scale is not finite
-      const float factor = at > position ? 0.f : vs;
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        const int d = min(i * 16 + m, dim - 1);
-        const uint4_t w = *(const uint4_t *)(vc + d * kBlock + 16 * g);
-        float4_t r = {};
-        r = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(w[0], w[1]), pf[0], r, 0, 0, 0);
-        r = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_codes(w[2], w[3]), pf[1], r, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(r[j], factor, o[i][j] * keep);
-      }
+      id = next_id, next_id = after;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -208,26 +239,26 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
     const bool whole = block0 == 0 && block1 == shape.blocks;
     const int slot = 2 * blockIdx.x + (unit == start ? 0 : 1);
     const int here = min(kRows, rows - tile * kRows);
-    for (int n = threadIdx.x; n < here * dim; n += kThreads) {
-      const int r = n / dim, d = n % dim;
-      float all = -__builtin_inff();
+    for (int r = wave; r < here; r += kWaves) {  // a wave has a row, a lane 4 dims
+      float all = -__builtin_inff(), weight = 0.f, f[kWaves];
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) all = fmaxf(all, stats[w * 2 * kRows + r]);
       const float zero_point = all == -__builtin_inff() ? 0.f : all;
-      float value = 0.f, weight = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(stats[w * 2 * kRows + r] - zero_point);
-        value += f * shared[(w * kRows + r) * (DP + 4) + d];
-        weight += f * stats[w * 2 * kRows + kRows + r];
+        f[w] = __builtin_amdgcn_exp2f(stats[w * 2 * kRows + r] - zero_point);
+        weight += f[w] * stats[w * 2 * kRows + kRows + r];
       }
+      const int d = lane * 4;
+      if (d >= dim) continue;
+      float4_t value = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) value += *(const float4_t *)(shared + (w * kRows + r) * (DP + 4) + d) * f[w];
       if (whole) {
-        const int at = tile * kRows + r;
-        half_t *to = a.out + (s.begin + at / a.group) * a.o_token + (int64_t)(h * a.group + at % a.group) * a.o_head;
-        to[d] = (half_t)(weight == 0.f ? 0.f : value / weight);
+        store_row(a, s, h, tile * kRows + r, d, value, weight);
       } else {
-        a.parts[((int64_t)slot * kRows + r) * dim + d] = value;
-        if (d == 0) {
+        *(float4_t *)(a.parts + ((int64_t)slot * kRows + r) * dim + d) = value;
+        if (lane == 0) {
           float *st = a.parts + (int64_t)2 * a.groups * kRows * dim + (int64_t)slot * 2 * kRows;
           st[r] = all, st[kRows + r] = weight;
         }
@@ -238,52 +269,280 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
   }
 }
 
+// ------------------------------------------------------------------------------------------------- many rows at a time
+//
+// kv_tile_kernel: prompts.  Bound by the matrix units: 4 dim operations for each row and key.  The products are turned as in
+// kv_split_kernel (S^T = K Q^T, O^T = V^T P^T, now 32x32x16), so that probabilities stay in their lanes: row 8 a + 4 g + b of a
+// key tile is token 16 g + 4 a + b, g = lane / 32, which makes a lane's 16 scores those of 16 consecutive tokens, in
+// the order of its 16 bytes of V^T.  Four waves with 32 rows each share a block's keys and values through LDS, where
+// they lie in binary16 in the order of the operands (1 KiB for a wave's load): every code is converted once a workgroup, not
+// once a wave.  The next block's bytes are loaded into registers before this block's products and converted behind them.
+//
+// Rescaling the accumulators for every block would cost as many vector instructions as the softmax.  The maximum in
+// use is only raised when scores pass it by more than 8 (probabilities up to 2^8 then), and the value scale enters the exponent
+// as its ratio to a reference, which only moves when the ratio leaves [1/16, 16]; the sum takes the ratio back out.
+
+constexpr int kTileThreads = 256, kTileRows = 128;
+
+__device__ __forceinline__ void store_codes(half_t *to, uint32_t lo, uint32_t hi) { *(half8_t *)to = eight_codes(lo, hi); }
+
+template <int DP>
+__global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel(AttentionArgs a) {
+  constexpr int kSteps = DP / 16;                    // of the product over dims
+  constexpr int kDimTiles = DP / 32;                 // of 32 dims of the result
+  constexpr int kRowsOfWave = 32, kRowsOfGroup = kTileRows;
+  constexpr int kHalves = kBlock * DP;               // binary16 of a block's keys (or values)
+  constexpr int kPieces = kBlock * DP / 16 / kTileThreads;  // 16-byte pieces of the keys (values) a thread stages
+  extern __shared__ half_t tile_shared[];  // [2][keys, values]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 31, g = lane >> 5;
+  const int dim = a.cache.dim, heads = a.cache.heads;
+
+  int b;
+  uint32_t base;
+  KvSequence s;
+  const auto units = [&](const KvSequence &s) { return (uint32_t)(s.count * a.group + kRowsOfGroup - 1) / kRowsOfGroup * heads; };
+  if (!kv_locate(a.batch, blockIdx.x, units, b, s, base)) return;
+  const int rows = s.count * a.group, tiles = (rows + kRowsOfGroup - 1) / kRowsOfGroup;
+  const int within = (int)(blockIdx.x - base), h = within % heads;
+  const int row0 = (tiles - 1 - within / heads) * kRowsOfGroup;  // the longest tiles first
+  const int *table = a.batch.table + (int64_t)b * a.batch.width;
+
+  // rows of this lane and of this wave
+  half8_t qf[kSteps];
+  int position;
+  const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
+  {
+    const int row = row0 + wave * kRowsOfWave + m;
+    const bool has_row = row < rows;
+    const int token = has_row ? row / a.group : 0, member = has_row ? row % a.group : 0;
+    position = has_row ? s.first + token : -1;
+    const half_t *q = a.q + (s.begin + token) * a.q_token + (int64_t)(h * a.group + member) * a.q_head;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      qf[k] = half8_t{};
+      if (has_row && k * 16 < dim) qf[k] = *(const half8_t *)(q + k * 16 + g * 8) * (half_t)sign;
+    }
+  }
+  const int wave_row = row0 + wave * kRowsOfWave;
+  const int wave_first = s.first + wave_row / a.group;                                          // its first row's position
+  const int wave_last = wave_row < rows ? s.first + (min(wave_row + kRowsOfWave, rows) - 1) / a.group : -1;
+  const int group_last = s.first + (min(row0 + kRowsOfGroup, rows) - 1) / a.group;
+  const int blocks = group_last < 0 ? 0 : group_last / kBlock + 1;
+
+  // staging: thread n has keys' piece (key, 16 dims c) and values' piece (dim d, 16 tokens)
+  uint4_t raw_k[kPieces], raw_v[kPieces];
+  float ks = 0.f, vs = 0.f;  // of the block that is staged
+  bool there = false;
+  const auto load = [&](int block) {
+    const int id = __builtin_amdgcn_readfirstlane(table[block]);
+    there = id >= 0 && id < a.cache.n_blocks;
+    if (!there) return;
+    const int64_t place = (int64_t)id * heads + h;
+    const uint8_t *kc = a.cache.k_codes + place * kBlock * dim, *vc = a.cache.v_codes + place * kBlock * dim;
+    ks = a.cache.k_scale[place], vs = a.cache.v_scale[place];
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int i = tid + n * kTileThreads, key = i / (DP / 16), c = i % (DP / 16), d = i / 4;
+      raw_k[n] = raw_v[n] = uint4_t{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // dims behind the last: zeros
+      if (c * 16 < dim) raw_k[n] = *(const uint4_t *)(kc + key * dim + c * 16);
+      if (d < dim) raw_v[n] = *(const uint4_t *)(vc + d * kBlock + i % 4 * 16);
+    }
+  };
+  // Keys: operand (tile T, step c) is 1 KiB, lane (g, row) has dims 16 c + 8 g ...; a row's two halves are stored by the thread
+  // that has its 16 dims.  The place within 512 bytes is turned by c, so that threads of one key and different c use
+  // different banks.  Values: operand (dim tile, T, u), lane (g, dim) has tokens 32 T + 16 g + 8 u ...
+  const auto stage = [&](int buffer) {
+    half_t *keys = tile_shared + buffer * 2 * kHalves, *vals = keys + kHalves;
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int i = tid + n * kTileThreads, key = i / (DP / 16), c = i % (DP / 16), d = i / 4, piece = i % 4;
+      const int in_tile = key & 31, row = (in_tile >> 2 & 3) * 8 + (in_tile >> 4) * 4 + (in_tile & 3);
+      half_t *to = keys + (((key >> 5) * kSteps + c) * 64 + (row ^ (c & 15))) * 8;
+      store_codes(to, raw_k[n][0], raw_k[n][1]);
+      store_codes(to + 32 * 8, raw_k[n][2], raw_k[n][3]);
+      half_t *tv = vals + (((d >> 5) * 4 + (piece >> 1) * 2) * 64 + (piece & 1) * 32 + (d & 31)) * 8;
+      store_codes(tv, raw_v[n][0], raw_v[n][1]);
+      store_codes(tv + 64 * 8, raw_v[n][2], raw_v[n][3]);
+    }
+  };
+
+  float16_t o[kDimTiles];
+  float most = -__builtin_inff(), sum = 0.f;
+  float reference = 1.f;
+#pragma unroll
+  for (int i = 0; i < kDimTiles; ++i) o[i] = float16_t{};
+  if (blocks > 0) {
+    load(0);
+    if (there) stage(0);
+  }
+  bool fresh = true;
+  for (int block = 0; block < blocks; ++block) {
+    __syncthreads();
+    const bool now = there;
+    const float key_scale = ks == 0.f ? 1.f : ks * fabsf(a.scale_log2), value_scale = vs;  // (keys of scale 0 are zeros)
+    if (block + 1 < blocks) load(block + 1);
+    const int at = block * kBlock;
+    if (now && at <= wave_last) {
+      const half_t *keys = tile_shared + (block & 1) * 2 * kHalves, *vals = keys + kHalves;
+      // the value scale against its reference
+      if (value_scale > 0.f && value_scale < __builtin_inff() && (fresh || value_scale > 16.f * reference || value_scale * 16.f < reference)) {
+        const float turn = fresh ? 1.f : reference / value_scale;
+        reference = value_scale, fresh = false;
+        if (turn != 1.f) {
+#pragma unroll
+          for (int i = 0; i < kDimTiles; ++i) o[i] *= turn;
+        }
+      }
+      const float ratio = value_scale == 0.f ? 1.f : value_scale / reference;
+      const bool masked = at + kBlock - 1 > wave_first;
+      float16_t score[2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        score[T] = float16_t{};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const half8_t kf = *(const half8_t *)(keys + ((T * kSteps + k) * 64 + g * 32 + (m ^ (k & 15))) * 8);
+          score[T] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[k], score[T], 0, 0, 0);
+        }
+      }
+      // a row that sees none of this block takes nothing from it, also where its scales are not finite
+      const bool none = at > position;
+      const float factor = none ? 1.f : key_scale, share = none ? 1.f : ratio;
+      float top = -__builtin_inff();
+      if (masked) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (at + T * 32 + 16 * g + i > position) score[T][i] = -__builtin_inff();
+      }
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, score[T][i]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * factor;
+      const bool raise = top > most + 8.f || (most == -__builtin_inff() && top > most);
+      if (__any(raise)) {
+        const float next = raise ? top : most;
+        const float keep = raise ? __builtin_amdgcn_exp2f(most - next) : 1.f;
+        most = next;
+        sum *= keep;
+#pragma unroll
+        for (int i = 0; i < kDimTiles; ++i) o[i] *= keep;
+      }
+      const float shift = __builtin_amdgcn_logf(share) - (most == -__builtin_inff() ? 0.f : most);
+      half8_t pf[2][2];
+      float part = 0.f;
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score[T][i], factor, shift));
+          part += p;
+          pf[T][i >> 3][i & 7] = (half_t)p;
+        }
+      sum += part / share;
+#pragma unroll
+      for (int i = 0; i < kDimTiles; ++i)
+#pragma unroll
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
+          }
+    }
+    if (block + 1 < blocks && there) stage((block + 1) & 1);
+  }
+  {
+    const float weight = sum + __shfl_xor(sum, 32);
+    const float factor = weight == 0.f ? 0.f : reference / weight;
+    const int row = row0 + wave * kRowsOfWave + m;
+    if (row >= rows) return;
+    half_t *to = a.out + (s.begin + row / a.group) * a.o_token + (int64_t)(h * a.group + row % a.group) * a.o_head;
+#pragma unroll
+    for (int i = 0; i < kDimTiles; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = i * 32 + c * 8 + g * 4;
+        if (d >= dim) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[d + j] = (half_t)(o[i][4 * c + j] * factor);
+      }
+  }
+}
+
 // Adds the parts of every (sequence, head, row tile) that more than one workgroup worked on.  Workgroup w of this grid has
 // boundary w + 1 of the cut; the first boundary inside a tile's units takes the tile.
 __global__ __launch_bounds__(kThreads) void kv_join_kernel(AttentionArgs a) {
-  const int dim = a.cache.dim;
-  const int64_t units = all_units(a), groups = active_groups(units, a.groups);
-  const int64_t w = blockIdx.x + 1;
-  if (units == 0 || w >= groups) return;
-  const int64_t unit = units * w / groups;
+  constexpr int kAhead = 4;
+  const int dim = a.cache.dim, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const auto units_of_sequence = [&](const KvSequence &s) { return units_of(a, s); };
+  const Cut cut(kv_units(a.batch, units_of_sequence), a.groups);
+  const uint32_t w = blockIdx.x + 1;
+  if (w >= cut.groups) return;
+  const uint32_t unit = cut.start(w);
   int b;
-  int64_t base;
-  if (!kv_locate(unit, a.batch.sequences, [&](int i) { return units_of(a, i); }, b, base)) return;
-  const KvSequence s = kv_sequence(a.batch, b);
+  uint32_t base;
+  KvSequence s;
+  if (!kv_locate(a.batch, unit, units_of_sequence, b, s, base)) return;
   const Shape shape = shape_of(a, s);
-  const int64_t which = (unit - base) / shape.blocks;
-  const int64_t from = base + which * shape.blocks, to = from + shape.blocks;
-  if (unit == from || units * (w - 1) / groups > from) return;
-  const int tile = (int)(which % shape.tiles), h = (int)(which / shape.tiles);
-  const int64_t last = (to * groups - 1) / units;  // the workgroup that has unit to - 1
-  const int here = min(kRows, s.count * a.group - tile * kRows);
+  const uint32_t which = (unit - base) / shape.blocks;
+  const uint32_t from = base + which * shape.blocks, to = from + shape.blocks;
+  if (unit == from || cut.start(w - 1) > from) return;
+  const int h = which / shape.tiles, tile = which - h * shape.tiles;
+  const int first = w - 1, last = cut.owner(to - 1);
+  const int here = min(kRows, s.count * a.group - tile * kRows), d = lane * 4;
   const float *stats = a.parts + (int64_t)2 * a.groups * kRows * dim;
-  for (int n = threadIdx.x; n < here * dim; n += kThreads) {
-    const int r = n / dim, d = n % dim;
-    float most = -__builtin_inff(), value = 0.f, weight = 0.f;
-    for (int64_t i = w - 1; i <= last; ++i) {
-      const int64_t slot = 2 * i + (units * i / groups < from ? 1 : 0);
-      const float m = stats[slot * 2 * kRows + r], l = stats[slot * 2 * kRows + kRows + r];
-      const float v = a.parts[(slot * kRows + r) * dim + d];
-      const float next = fmaxf(most, m), zero_point = next == -__builtin_inff() ? 0.f : next;
-      const float keep = __builtin_amdgcn_exp2f(most - zero_point), f = __builtin_amdgcn_exp2f(m - zero_point);
-      value = value * keep + v * f, weight = weight * keep + l * f, most = next;
+  for (int r = wave; r < here; r += kThreads / 64) {
+    if (d >= dim) continue;
+    float most = -__builtin_inff(), weight = 0.f;
+    float4_t value = {};
+    for (int i = first; i <= last; i += kAhead) {
+      float m[kAhead], l[kAhead];
+      float4_t v[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        // (the part of a workgroup that starts before this tile is its second one; behind the last: nothing)
+        const int64_t slot = 2 * min(i + n, last) + (i + n == first && cut.start(first) < from ? 1 : 0);
+        m[n] = stats[slot * 2 * kRows + r], l[n] = stats[slot * 2 * kRows + kRows + r];
+        v[n] = *(const float4_t *)(a.parts + (slot * kRows + r) * dim + d);
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        if (i + n > last) break;
+        const float next = fmaxf(most, m[n]), zero_point = next == -__builtin_inff() ? 0.f : next;
+        const float keep = __builtin_amdgcn_exp2f(most - zero_point), f = __builtin_amdgcn_exp2f(m[n] - zero_point);
+        value = value * keep + v[n] * f, weight = weight * keep + l[n] * f, most = next;
+      }
     }
-    const int at = tile * kRows + r;
-    half_t *o = a.out + (s.begin + at / a.group) * a.o_token + (int64_t)(h * a.group + at % a.group) * a.o_head;
-    o[d] = (half_t)(weight == 0.f ? 0.f : value / weight);
+    store_row(a, s, h, tile * kRows + r, d, value, weight);
   }
+}
+
+// A kernel has to be told of more than 64 KiB of LDS, on each device.
+int allow_lds(const void *kernel, size_t bytes, const char *who) {
+  if (bytes <= 64 << 10) return GQ_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? GQ_OK : fail((int)e, "%s: %s", who, hipGetErrorString(e));
 }
 
 template <int DP>
 int launch_split(const AttentionArgs &a, hipStream_t stream) {
   const size_t lds = (size_t)kWaves * kRows * (DP + 4 + 2) * sizeof(float);
-  if (lds > 64 << 10) {
-    const hipError_t e = hipFuncSetAttribute((const void *)kv_split_kernel<DP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return fail((int)e, "kv_split_kernel: %s", hipGetErrorString(e));
-  }
+  if (const int rc = allow_lds((const void *)kv_split_kernel<DP>, lds, "kv_split_kernel")) return rc;
   kv_split_kernel<DP><<<a.groups, kThreads, lds, stream>>>(a);
   return check_launch("kv_split_kernel");
+}
+
+template <int DP>
+int launch_tile(const AttentionArgs &a, hipStream_t stream) {
+  const size_t lds = (size_t)2 * 2 * kBlock * DP * sizeof(half_t);
+  if (const int rc = allow_lds((const void *)kv_tile_kernel<DP>, lds, "kv_tile_kernel")) return rc;
+  const int64_t groups = a.cache.heads * ((int64_t)a.batch.tokens * a.group / kTileRows + a.batch.sequences);
+  if (groups > 0x7fffffff) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16: too many rows for one launch");
+  kv_tile_kernel<DP><<<(unsigned)groups, kTileThreads, lds, stream>>>(a);
+  return check_launch("kv_tile_kernel");
 }
 
 }  // namespace
@@ -303,6 +562,13 @@ int launch_kv_attention(const KvCache &cache, const KvBatch &batch, const uint16
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.parts = (float *)workspace;
   a.groups = kMostGroups;
+  // Both kernels are right for every batch; which is faster goes by the rows of a sequence and kv head, on average.
+  // (The units of kv_split_kernel have to be countable in 31 bits.)
+  const double most_units = (double)cache.heads * ((double)batch.tokens * a.group / kRows + batch.sequences) * (batch.width + 1);
+  if (most_units >= 2147483648. || (int64_t)batch.tokens * a.group >= (int64_t)kTileLeast * batch.sequences)
+    return cache.dim <= 64    ? launch_tile<64>(a, stream)
+           : cache.dim <= 128 ? launch_tile<128>(a, stream)
+                              : launch_tile<256>(a, stream);
   int rc = cache.dim <= 64 ? launch_split<64>(a, stream) : cache.dim <= 128 ? launch_split<128>(a, stream) : launch_split<256>(a, stream);
   if (rc != GQ_OK) return rc;
   kv_join_kernel<<<a.groups - 1, kThreads, 0, stream>>>(a);

@@ -37,16 +37,15 @@ struct Place {
   int row, slot, count, position, id;
 };
 
-__device__ __forceinline__ bool find_place(const KvCache &cache, const KvBatch &batch, int64_t unit, Place &p) {
+__device__ __forceinline__ bool find_place(const KvCache &cache, const KvBatch &batch, uint32_t unit, Place &p) {
   int b;
-  int64_t base;
-  const auto units = [&](int i) {
-    const KvSequence s = kv_sequence(batch, i);
+  uint32_t base;
+  KvSequence s;
+  const auto units = [&](const KvSequence &s) {
     const int from = max(s.first, 0);
-    return s.length > from ? (s.length - 1) / kBlock - from / kBlock + 1 : 0;
+    return (uint32_t)(s.length > from ? (s.length - 1) / kBlock - from / kBlock + 1 : 0);
   };
-  if (!kv_locate(unit, batch.sequences, units, b, base)) return false;
-  const KvSequence s = kv_sequence(batch, b);
+  if (!kv_locate(batch, unit, units, b, s, base)) return false;
   const int from = max(s.first, 0), block = from / kBlock + (int)(unit - base);
   p.position = max(from, block * kBlock);
   p.slot = p.position - block * kBlock;
