@@ -15,13 +15,20 @@ BLOCK = 64  # tokens of one block of the cache, the unit that has a scale of its
 BASE = 10000.0
 
 
-def _framework():
-    path = os.path.join(os.getcwd(), "popxl-addons_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    from popxl_addons import ops
+_ops = None
 
-    return ops
+
+def _framework():
+    """popxl_addons.ops, imported at the first call (a program imports it once, not with every call of an operator)."""
+    global _ops
+    if _ops is None:
+        path = os.path.join(os.getcwd(), "popxl-addons_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        from popxl_addons import ops
+
+        _ops = ops
+    return _ops
 
 
 # ------------------------------------------------------------------------------------------------- cases
