@@ -55,12 +55,14 @@ __device__ __forceinline__ uint32_t units_of(const AttentionArgs &a, const KvSeq
   return (uint32_t)shape.tiles * shape.blocks * a.cache.heads;
 }
 
-// The cut of the units: `groups` workgroups take part, enough that each has four blocks, one for each wave; the first `more` of
-// them have one unit more than the others.
+// The cut of the units: `groups` workgroups take part, the first `more` of them with one unit more than the others.  Up to 256
+// units every one has a workgroup, and so a compute unit, of its own: what a compute unit gets from memory is what a short
+// history waits for (13 blocks x 16 heads of 256: 9 us, with a block for each wave of 52 workgroups 15 us).  More units make
+// workgroups of four, one for each wave.
 struct Cut {
   uint32_t units, groups, each, more;
   __device__ Cut(uint32_t units_, uint32_t most) : units(units_) {
-    const uint32_t want = (units + kWaves - 1) / kWaves;
+    const uint32_t want = max(min(units, 256u), (units + kWaves - 1) / kWaves);
     groups = min(max(want, 1u), most);
     each = units / groups, more = units - each * groups;
   }
@@ -494,29 +496,44 @@ __global__ __launch_bounds__(kThreads) void kv_join_kernel(AttentionArgs a) {
   const int first = w - 1, last = cut.owner(to - 1);
   const int here = min(kRows, s.count * a.group - tile * kRows), d = lane * 4;
   const float *stats = a.parts + (int64_t)2 * a.groups * kRows * dim;
-  for (int r = wave; r < here; r += kThreads / 64) {
-    if (d >= dim) continue;
+  // a wave has a row, or, of few rows, every fourth part of each
+  __shared__ float4_t values[kWaves][64];
+  __shared__ float maxima[kWaves], weights[kWaves];
+  const bool alone = here >= kWaves;
+  for (int r = alone ? wave : 0; r < here; r += alone ? kWaves : 1) {
     float most = -__builtin_inff(), weight = 0.f;
     float4_t value = {};
-    for (int i = first; i <= last; i += kAhead) {
+    const auto add = [&](float m, float l, float4_t v) {
+      const float next = fmaxf(most, m), zero_point = next == -__builtin_inff() ? 0.f : next;
+      const float keep = __builtin_amdgcn_exp2f(most - zero_point), f = __builtin_amdgcn_exp2f(m - zero_point);
+      value = value * keep + v * f, weight = weight * keep + l * f, most = next;
+    };
+    const int step = alone ? 1 : kWaves;
+    for (int i = first + (alone ? 0 : wave); i <= last; i += kAhead * step) {
       float m[kAhead], l[kAhead];
       float4_t v[kAhead];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) {
         // (the part of a workgroup that starts before this tile is its second one; behind the last: nothing)
-        const int64_t slot = 2 * min(i + n, last) + (i + n == first && cut.start(first) < from ? 1 : 0);
+        const int part = min(i + n * step, last);
+        const int64_t slot = 2 * part + (part == first && cut.start(first) < from ? 1 : 0);
         m[n] = stats[slot * 2 * kRows + r], l[n] = stats[slot * 2 * kRows + kRows + r];
-        v[n] = *(const float4_t *)(a.parts + (slot * kRows + r) * dim + d);
+        v[n] = d < dim ? *(const float4_t *)(a.parts + (slot * kRows + r) * dim + d) : float4_t{};
       }
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        if (i + n > last) break;
-        const float next = fmaxf(most, m[n]), zero_point = next == -__builtin_inff() ? 0.f : next;
-        const float keep = __builtin_amdgcn_exp2f(most - zero_point), f = __builtin_amdgcn_exp2f(m[n] - zero_point);
-        value = value * keep + v[n] * f, weight = weight * keep + l[n] * f, most = next;
-      }
+      for (int n = 0; n < kAhead; ++n)
+        if (i + n * step <= last) add(m[n], l[n], v[n]);
     }
-    store_row(a, s, h, tile * kRows + r, d, value, weight);
+    if (!alone) {
+      __syncthreads();
+      values[wave][lane] = value;
+      if (lane == 0) maxima[wave] = most, weights[wave] = weight;
+      __syncthreads();
+      if (wave > 0) continue;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) add(maxima[w], weights[w], values[w][lane]);
+    }
+    if (d < dim) store_row(a, s, h, tile * kRows + r, d, value, weight);
   }
 }
 

@@ -199,10 +199,21 @@ def last_error():
 
 def call(name, *args):
     """Call an entry point; raise GQHipError on a non-zero return."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         raise GQHipError(name, rc, lib.gq_last_error().decode("utf-8", "replace"))
+
+
+def launch(index, name, *args):
+    """Call an entry point whose last argument is the stream, on the current stream of HIP device `index`, with that device
+    current (the guard costs as much as a launch, so it is entered only where it changes something)."""
+    import torch
+
+    if torch.cuda.current_device() == index:
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 _kn_workspaces = {}

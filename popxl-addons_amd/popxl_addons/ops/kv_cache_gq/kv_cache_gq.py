@@ -67,46 +67,48 @@ class KVCacheGQ:
     def _adopt(self, k_codes, v_codes, k_scale, v_scale):
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.n_blocks, self.kv_heads, _, self.head_dim = k_codes.shape
+        self.device, self.index = k_codes.device, k_codes.get_device()
         self._c = _gq_hip.KvCache(*(t.data_ptr() for t in (k_codes, v_codes, k_scale, v_scale)), self.n_blocks, self.kv_heads,
                                   self.head_dim)
-
-    @property
-    def device(self):
-        return self.k_codes.device
+        self._attention_workspace = _gq_hip.load().gq_kv_attention_workspace_bytes(self.head_dim)
 
 
 def _batch(cache, offsets, seq_lens, block_table, tokens):
     """The batch for the C entry points, and the tensors to keep until the call has been made."""
     import torch
 
-    if not cache.device.type == "cuda":
+    index = cache.index
+    if index < 0:
         raise RuntimeError("the key/value cache runs on the GPU only: make it on a HIP device")
     for name, t in (("offsets", offsets), ("seq_lens", seq_lens), ("block_table", block_table)):
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32, got {t.dtype}")
-        if t.device != cache.device:
+        if t.get_device() != index:
             raise ValueError(f"{name} must be on the cache's device")
-    if seq_lens.dim() != 1 or tuple(offsets.shape) != (seq_lens.shape[0] + 1,):
+    sequences = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    if sequences < 0 or offsets.dim() != 1 or offsets.shape[0] != sequences + 1:
         raise ValueError(f"offsets must have one entry more than seq_lens, got {tuple(offsets.shape)} and {tuple(seq_lens.shape)}")
-    if block_table.dim() != 2 or block_table.shape[0] != seq_lens.shape[0]:
-        raise ValueError(f"block_table must be [{seq_lens.shape[0]}, blocks], got {tuple(block_table.shape)}")
-    keep = offsets.contiguous(), seq_lens.contiguous(), block_table.contiguous()
-    return _gq_hip.KvBatch(*(t.data_ptr() for t in keep), seq_lens.shape[0], block_table.shape[1], tokens), keep
+    if block_table.dim() != 2 or block_table.shape[0] != sequences:
+        raise ValueError(f"block_table must be [{sequences}, blocks], got {tuple(block_table.shape)}")
+    offsets, seq_lens, block_table = keep = offsets.contiguous(), seq_lens.contiguous(), block_table.contiguous()
+    return _gq_hip.KvBatch(offsets.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), sequences, block_table.shape[1], tokens), keep
 
 
 def _rows(name, t, cache, heads):
-    """t [tokens, heads, head_dim] float16 with rows that the kernels can load (a copy where they cannot)."""
+    """t [tokens, heads, head_dim] float16 with rows that the kernels can load (a copy where they cannot), and its strides."""
     import torch
 
     if t.dim() != 3 or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads if heads is not None else 'heads'}, {cache.head_dim}], got {tuple(t.shape)}")
     if t.dtype != torch.float16:
         raise TypeError(f"{name} must be float16, got {t.dtype}")
-    if t.device != cache.device:
+    if t.get_device() != cache.index:
         raise ValueError(f"{name} must be on the cache's device")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    token_stride, head_stride, stride = t.stride()
+    if stride != 1 or token_stride % 8 or head_stride % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        token_stride, head_stride, _ = t.stride()
+    return t, token_stride, head_stride
 
 
 def kv_cache_append(cache, k, v, offsets, seq_lens, block_table, rotary=None):
@@ -123,21 +125,18 @@ def kv_cache_append(cache, k, v, offsets, seq_lens, block_table, rotary=None):
     A block that starts with these tokens gets the scale amax / 127.  In a block that has tokens the scale grows, where it must,
     by a power of two, and the codes there are scaled down by it: every value stays within one scale of what was stored.
     """
-    import torch
-
     batch, keep = _batch(cache, offsets, seq_lens, block_table, k.shape[0])
-    if tuple(k.shape) != tuple(v.shape):
+    if k.shape != v.shape:
         raise ValueError(f"k and v must have the same shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    k, v = _rows("k", k, cache, cache.kv_heads), _rows("v", v, cache, cache.kv_heads)
+    k, k_token_stride, k_head_stride = _rows("k", k, cache, cache.kv_heads)
+    v, v_token_stride, v_head_stride = _rows("v", v, cache, cache.kv_heads)
     if rotary is not None:
-        if rotary.turns.device != cache.device:
+        if rotary.index != cache.index:
             raise ValueError("rotary must be on the cache's device")
         if rotary.rotary_dim > cache.head_dim:
             raise ValueError(f"rotary_dim={rotary.rotary_dim} exceeds the head dimension {cache.head_dim}")
-    with torch.cuda.device(cache.device):
-        _gq_hip.call("gq_kv_append_f16", ctypes.byref(cache._c), ctypes.byref(batch), k.data_ptr(), k.stride(0), k.stride(1),
-                     v.data_ptr(), v.stride(0), v.stride(1), None if rotary is None else rotary.argument,
-                     torch.cuda.current_stream(cache.device).cuda_stream)
+    _gq_hip.launch(cache.index, "gq_kv_append_f16", ctypes.byref(cache._c), ctypes.byref(batch), k.data_ptr(), k_token_stride,
+                   k_head_stride, v.data_ptr(), v_token_stride, v_head_stride, None if rotary is None else rotary.argument)
 
 
 def kv_cache_gather(cache, offsets, seq_lens, block_table, tokens, out=None):
@@ -150,14 +149,13 @@ def kv_cache_gather(cache, offsets, seq_lens, block_table, tokens, out=None):
 
     batch, keep = _batch(cache, offsets, seq_lens, block_table, tokens)
     shape = (tokens, cache.kv_heads, cache.head_dim)
-    with torch.cuda.device(cache.device):
-        if out is None:
-            out = tuple(torch.empty(shape, dtype=torch.float16, device=cache.device) for _ in range(2))
-        for t in out:
-            if tuple(t.shape) != shape or not t.is_contiguous() or t.dtype != torch.float16 or t.device != cache.device:
-                raise ValueError(f"out must be two contiguous float16 tensors of shape {shape} on the cache's device")
-        _gq_hip.call("gq_kv_gather_f16", ctypes.byref(cache._c), ctypes.byref(batch), out[0].data_ptr(), out[1].data_ptr(),
-                     torch.cuda.current_stream(cache.device).cuda_stream)
+    if out is None:
+        out = (torch.empty(shape, dtype=torch.float16, device=cache.device), torch.empty(shape, dtype=torch.float16, device=cache.device))
+    k, v = out
+    for t in out:
+        if t.shape != shape or not t.is_contiguous() or t.dtype != torch.float16 or t.get_device() != cache.index:
+            raise ValueError(f"out must be two contiguous float16 tensors of shape {shape} on the cache's device")
+    _gq_hip.launch(cache.index, "gq_kv_gather_f16", ctypes.byref(cache._c), ctypes.byref(batch), k.data_ptr(), v.data_ptr())
     return out
 
 
@@ -178,21 +176,21 @@ def kv_cache_attention(q, cache, offsets, seq_lens, block_table, scale=None, out
     import torch
 
     batch, keep = _batch(cache, offsets, seq_lens, block_table, q.shape[0])
-    q = _rows("q", q, cache, None)
-    if q.shape[1] % cache.kv_heads != 0:
-        raise ValueError(f"q has {q.shape[1]} heads, not a multiple of the cache's {cache.kv_heads}")
-    if out is not None:
-        if out.shape != q.shape or out.stride(2) != 1 or out.device != q.device:
-            raise ValueError("out must have the shape and device of q and a contiguous last axis")
-        if out.dtype != torch.float16:
-            raise TypeError("out must be float16")
-    with torch.cuda.device(cache.device):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if q.shape[1] == 0:
-            return out
-        workspace = torch.empty(_gq_hip.load().gq_kv_attention_workspace_bytes(cache.head_dim), dtype=torch.uint8, device=q.device)
-        _gq_hip.call("gq_kv_attention_f16", ctypes.byref(cache._c), ctypes.byref(batch), q.data_ptr(), q.stride(0), q.stride(1),
-                     out.data_ptr(), out.stride(0), out.stride(1), q.shape[1], cache.head_dim ** -0.5 if scale is None else scale,
-                     workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream(q.device).cuda_stream)
+    q, q_token_stride, q_head_stride = _rows("q", q, cache, None)
+    shape = q.shape
+    if shape[1] % cache.kv_heads != 0:
+        raise ValueError(f"q has {shape[1]} heads, not a multiple of the cache's {cache.kv_heads}")
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.stride(2) != 1 or out.get_device() != cache.index:
+        raise ValueError("out must have the shape and device of q and a contiguous last axis")
+    elif out.dtype != torch.float16:
+        raise TypeError("out must be float16")
+    if shape[1] == 0:
+        return out
+    token_stride, head_stride, _ = out.stride()
+    workspace = torch.empty(cache._attention_workspace, dtype=torch.uint8, device=cache.device)
+    _gq_hip.launch(cache.index, "gq_kv_attention_f16", ctypes.byref(cache._c), ctypes.byref(batch), q.data_ptr(), q_token_stride,
+                   q_head_stride, out.data_ptr(), token_stride, head_stride, shape[1], cache.head_dim ** -0.5 if scale is None else scale,
+                   workspace.data_ptr(), cache._attention_workspace)
     return out

@@ -38,12 +38,24 @@ class LowRankAdapters:
         self.down, self.up, self.scaling = down, up, scaling
         self.n_adapters, self.rank, self.in_features = down.shape
         self.out_features = up.shape[1]
+        self.device, self.index = down.device, down.get_device()
+        self._workspaces = {}  # bytes that a call needs, by entry point and rows
         self._c = _gq_hip.Adapters(down.data_ptr(), up.data_ptr(), scaling.data_ptr(), self.n_adapters, self.rank, self.in_features,
                                    self.out_features)
 
-    @property
-    def device(self):
-        return self.down.device
+    def workspace(self, function, rows):
+        """A new workspace for a call over `rows` rows (one that the allocator orders with the stream it is used on)."""
+        import torch
+
+        need = self._workspaces.get((function, rows))
+        if need is None:
+            need = getattr(_gq_hip.load(), function)(ctypes.byref(self._c), rows)
+            if need < 0:
+                raise _gq_hip.GQHipError(function, need, _gq_hip.last_error())
+            if len(self._workspaces) > 256:
+                self._workspaces.clear()
+            self._workspaces[function, rows] = need
+        return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
 
 class AdapterPlan:
@@ -59,7 +71,7 @@ class AdapterPlan:
             raise ValueError(f"AdapterPlan: {n_adapters} adapters outside 1 ... 2048")
         if ids.dim() != 1:
             raise ValueError(f"AdapterPlan: ids must be [rows], got {tuple(ids.shape)}")
-        self.rows, self.n_adapters, self.device = ids.shape[0], n_adapters, ids.device
+        self.rows, self.n_adapters, self.device, self.index = ids.shape[0], n_adapters, ids.device, ids.get_device()
         nbytes = _gq_hip.load().gq_adapter_plan_bytes(self.rows, n_adapters)
         if nbytes < 0:
             raise _gq_hip.GQHipError("gq_adapter_plan_bytes", nbytes, _gq_hip.last_error())
@@ -72,12 +84,10 @@ class AdapterPlan:
 
         if ids.dtype != torch.int32:
             raise TypeError(f"AdapterPlan: ids must be int32, got {ids.dtype}")
-        if tuple(ids.shape) != (self.rows,) or ids.device != self.device:
+        if ids.dim() != 1 or ids.shape[0] != self.rows or ids.get_device() != self.index:
             raise ValueError(f"AdapterPlan: ids must be [{self.rows}] on {self.device}")
         ids = ids.contiguous()
-        with torch.cuda.device(self.device):
-            _gq_hip.call("gq_adapter_plan", ids.data_ptr(), self.rows, self.n_adapters, self.data.data_ptr(), self.data.numel(),
-                         torch.cuda.current_stream(self.device).cuda_stream)
+        _gq_hip.launch(self.index, "gq_adapter_plan", ids.data_ptr(), self.rows, self.n_adapters, self.data.data_ptr(), self.data.numel())
 
 
 def _matrix(name, t, features, adapters, rows):
@@ -90,7 +100,7 @@ def _matrix(name, t, features, adapters, rows):
         raise TypeError(f"{name} must be float16, got {t.dtype}")
     if t.shape[-1] != features:
         raise ValueError(f"{name} must have {features} features, got {t.shape[-1]}")
-    if t.device != adapters.device:
+    if t.get_device() != adapters.index:
         raise ValueError(f"{name} must be on the adapters' device")
     if t.dim() != 2 or t.stride(1) != 1:
         t = t.reshape(-1, features).contiguous()
@@ -100,17 +110,8 @@ def _matrix(name, t, features, adapters, rows):
 
 
 def _check_plan(adapters, plan):
-    if plan.n_adapters != adapters.n_adapters or plan.device != adapters.device:
+    if plan.n_adapters != adapters.n_adapters or plan.index != adapters.index:
         raise ValueError(f"the plan is for {plan.n_adapters} adapters on {plan.device}, these are {adapters.n_adapters} on {adapters.device}")
-
-
-def _workspace(function, adapters, rows):
-    import torch
-
-    need = getattr(_gq_hip.load(), function)(ctypes.byref(adapters._c), rows)
-    if need < 0:
-        raise _gq_hip.GQHipError(function, need, _gq_hip.last_error())
-    return torch.empty(need, dtype=torch.uint8, device=adapters.device)
 
 
 def low_rank_adapters(x, y, adapters, plan, activation=None, out=None):
@@ -130,23 +131,21 @@ def low_rank_adapters(x, y, adapters, plan, activation=None, out=None):
     """
     import torch
 
-    act = _gq_hip.activation_code(activation)
+    act, rows, features = _gq_hip.activation_code(activation), plan.rows, adapters.out_features
     _check_plan(adapters, plan)
-    x2 = _matrix("x", x, adapters.in_features, adapters, plan.rows)
-    shape = (*x.shape[:-1], adapters.out_features)
-    y2 = None if y is None else _matrix("y", y, adapters.out_features, adapters, plan.rows)
-    with torch.cuda.device(adapters.device):
-        if out is None:
-            out = torch.empty(shape, dtype=torch.float16, device=adapters.device)
-        if out.dtype != torch.float16 or out.shape[-1] != adapters.out_features or out.device != adapters.device:
-            raise ValueError(f"out must be float16 [..., {adapters.out_features}] on the adapters' device")
-        out2 = out if out.dim() == 2 and out.stride(1) == 1 else out.view(-1, adapters.out_features)
-        if out2.shape[0] != plan.rows:
-            raise ValueError(f"out has {out2.shape[0]} rows, the plan {plan.rows}")
-        workspace = _workspace("gq_adapter_apply_workspace_bytes", adapters, plan.rows)
-        _gq_hip.call("gq_adapter_apply_f16", ctypes.byref(adapters._c), plan.data.data_ptr(), plan.rows, x2.data_ptr(), x2.stride(0),
-                     0 if y2 is None else y2.data_ptr(), 0 if y2 is None else y2.stride(0), out2.data_ptr(), out2.stride(0), act,
-                     workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream(adapters.device).cuda_stream)
+    x2 = _matrix("x", x, adapters.in_features, adapters, rows)
+    y2 = None if y is None else _matrix("y", y, features, adapters, rows)
+    if out is None:
+        out = x.new_empty((*x.shape[:-1], features))
+    elif out.dtype != torch.float16 or out.shape[-1] != features or out.get_device() != adapters.index:
+        raise ValueError(f"out must be float16 [..., {features}] on the adapters' device")
+    out2 = out if out.dim() == 2 and out.stride(1) == 1 else out.view(-1, features)
+    if out2.shape[0] != rows:
+        raise ValueError(f"out has {out2.shape[0]} rows, the plan {rows}")
+    workspace, nbytes = adapters.workspace("gq_adapter_apply_workspace_bytes", rows)
+    _gq_hip.launch(adapters.index, "gq_adapter_apply_f16", ctypes.byref(adapters._c), plan.data.data_ptr(), rows, x2.data_ptr(), x2.stride(0),
+                   0 if y2 is None else y2.data_ptr(), 0 if y2 is None else y2.stride(0), out2.data_ptr(), out2.stride(0), act,
+                   workspace.data_ptr(), nbytes)
     return out
 
 
@@ -168,16 +167,13 @@ def low_rank_adapters_grad(x, dy, adapters, plan, dx=None):
     x2 = _matrix("x", x, adapters.in_features, adapters, plan.rows)
     dy2 = _matrix("dy", dy, adapters.out_features, adapters, plan.rows)
     dx2 = None if dx is None else _matrix("dx", dx, adapters.in_features, adapters, plan.rows)
-    with torch.cuda.device(adapters.device):
-        out = torch.empty(x.shape, dtype=torch.float16, device=adapters.device)
-        shapes = (adapters.down.shape, adapters.up.shape)
-        if plan.rows == 0 or adapters.in_features == 0 or adapters.out_features == 0:
-            d_down, d_up = (torch.zeros(s, dtype=torch.float32, device=adapters.device) for s in shapes)
-            return out if dx is None else out.copy_(dx), d_down, d_up
-        d_down, d_up = (torch.empty(s, dtype=torch.float32, device=adapters.device) for s in shapes)
-        workspace = _workspace("gq_adapter_grad_workspace_bytes", adapters, plan.rows)
-        _gq_hip.call("gq_adapter_grad_f16", ctypes.byref(adapters._c), plan.data.data_ptr(), plan.rows, x2.data_ptr(), x2.stride(0),
-                     dy2.data_ptr(), dy2.stride(0), 0 if dx2 is None else dx2.data_ptr(), 0 if dx2 is None else dx2.stride(0),
-                     out.data_ptr(), adapters.in_features, d_down.data_ptr(), d_up.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                     torch.cuda.current_stream(adapters.device).cuda_stream)
+    out = x.new_empty(x.shape)
+    if plan.rows == 0 or adapters.in_features == 0 or adapters.out_features == 0:
+        d_down, d_up = (torch.zeros(w.shape, dtype=torch.float32, device=w.device) for w in (adapters.down, adapters.up))
+        return out if dx is None else out.copy_(dx), d_down, d_up
+    d_down, d_up = (torch.empty(w.shape, dtype=torch.float32, device=w.device) for w in (adapters.down, adapters.up))
+    workspace, nbytes = adapters.workspace("gq_adapter_grad_workspace_bytes", plan.rows)
+    _gq_hip.launch(adapters.index, "gq_adapter_grad_f16", ctypes.byref(adapters._c), plan.data.data_ptr(), plan.rows, x2.data_ptr(),
+                   x2.stride(0), dy2.data_ptr(), dy2.stride(0), 0 if dx2 is None else dx2.data_ptr(), 0 if dx2 is None else dx2.stride(0),
+                   out.data_ptr(), adapters.in_features, d_down.data_ptr(), d_up.data_ptr(), workspace.data_ptr(), nbytes)
     return out, d_down, d_up

@@ -72,6 +72,7 @@ class RotaryPosEmbed:
         frequencies, self.factor = rotary_frequencies(rotary_dim, base, scaling)
         self.rotary_dim, self.layout = rotary_dim, layout
         self.turns = torch.from_numpy(frequencies / (2 * math.pi)).to(device)
+        self.index = self.turns.get_device()
         self._c = _gq_hip.Rotary(self.turns.data_ptr(), self.factor, rotary_dim, _LAYOUTS[layout])
 
     @property
@@ -105,20 +106,23 @@ def rotary_pos_embed(t, positions, rotary, inverse=False, out=None):
         raise TypeError("rotary_pos_embed: t and out must be float16")
     if positions.dtype != torch.int32:
         raise TypeError(f"rotary_pos_embed: positions must be int32, got {positions.dtype}")
-    if tuple(positions.shape) != (t.shape[0],):
-        raise ValueError(f"positions must have shape ({t.shape[0]},), got {tuple(positions.shape)}")
-    if positions.device != t.device or rotary.turns.device != t.device or (out is not None and out.device != t.device):
+    index, shape = t.get_device(), t.shape
+    tokens, heads, head_dim = shape
+    if positions.dim() != 1 or positions.shape[0] != tokens:
+        raise ValueError(f"positions must have shape ({tokens},), got {tuple(positions.shape)}")
+    if positions.get_device() != index or rotary.index != index or (out is not None and out.get_device() != index):
         raise ValueError("t, positions, rotary and out must be on the same device")
-    if rotary.rotary_dim > t.shape[2]:
-        raise ValueError(f"rotary_dim={rotary.rotary_dim} exceeds the head dimension {t.shape[2]}")
-    if out is not None and (out.shape != t.shape or out.stride(2) != 1):
+    if rotary.rotary_dim > head_dim:
+        raise ValueError(f"rotary_dim={rotary.rotary_dim} exceeds the head dimension {head_dim}")
+    if out is not None and (out.shape != shape or out.stride(2) != 1):
         raise ValueError("out must have the shape of t and a contiguous last axis")
     if t.stride(2) != 1:
         t = t.contiguous()
     positions = positions.contiguous()
-    with torch.cuda.device(t.device):
-        if out is None:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        _gq_hip.call("gq_rotary_f16", t.data_ptr(), t.stride(0), t.stride(1), positions.data_ptr(), rotary.argument, int(inverse),
-                     out.data_ptr(), out.stride(0), out.stride(1), *t.shape, torch.cuda.current_stream(t.device).cuda_stream)
+    if out is None:
+        out = t.new_empty(shape)
+    token_stride, head_stride, _ = t.stride()
+    out_token_stride, out_head_stride, _ = out.stride()
+    _gq_hip.launch(index, "gq_rotary_f16", t.data_ptr(), token_stride, head_stride, positions.data_ptr(), rotary.argument, inverse,
+                   out.data_ptr(), out_token_stride, out_head_stride, tokens, heads, head_dim)
     return out
