@@ -7,10 +7,12 @@
 // < s.  (With s following amax / 127 itself, every token that sets a new maximum would add another half step.)
 // Codes are rint(x / s) with the correctly rounded quotient: a plain binary32 program gets the same codes.
 //
-// Bound by HBM: 2 bytes read and 1 written an element.  A workgroup owns one (block, head) of the keys or of the values: the
-// scale is a maximum over all of it, and no other workgroup writes there.  Its 256 threads hold the new tokens in registers
-// as pieces of 4 tokens x 8 dims: 16-byte loads that are contiguous over the row, 8-byte stores of key codes, and for the
-// transposed value codes a 4-byte word of 4 tokens for each dim, which goes through LDS to 16-byte stores.
+// Bound by HBM: 2 bytes read and 1 written an element.  A workgroup owns a (block, head) of the keys or of the values: the
+// scale is a maximum over all of it, and no other workgroup writes there.  The new tokens come by 16-byte loads that are
+// contiguous over a row and wait in LDS, as binary16, for the scale; from there key codes go out 8 dims at a time, and value
+// codes, which the cache holds transposed, 16 tokens of a dim at a time.  Keys that are turned on the way: the angles of the
+// block's tokens are formed once in LDS and serve several heads.  (With the tokens held in registers instead the kernel had 160
+// of them and 23 KiB of code, and a decode step waited for its instructions: 19 us for 48 requests.)
 #include "gq_kv.h"
 #include "gq_rotary.h"
 
@@ -18,8 +20,7 @@ namespace gq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxDim = 256;
-constexpr int kPieces = 16 * (kMaxDim / 8) / kThreads;  // pieces of 4 tokens x 8 dims a thread holds at most
+constexpr int kFew = 8;  // new tokens of a block up to which their value codes are stored byte by byte
 
 struct AppendArgs {
   KvCache cache;
@@ -28,7 +29,8 @@ struct AppendArgs {
   int64_t token[2], head[2];
   const double *turns;  // NULL: keys are stored as they come
   float factor;
-  int rotary_dim;
+  int rotary_dim, heads_per_group;
+  int first;  // blockIdx.y + first: 0 keys, 1 values
   bool half_layout;
 };
 
@@ -55,169 +57,220 @@ __device__ __forceinline__ bool find_place(const KvCache &cache, const KvBatch &
   return p.id >= 0 && p.id < cache.n_blocks;
 }
 
-__device__ __forceinline__ uint32_t quantise(half_t x, float scale) {
-  if (!(scale > 0.f)) return 128;  // a block of zeros
-  const float q = rintf((float)x / scale);
-  return (uint32_t)(int)(fminf(fmaxf(q, -127.f), 127.f) + 128.f);  // (fmaxf maps a NaN, of an infinite block, to -127)
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+
+// What turns values into codes at one scale: rint of the correctly rounded binary32 quotient.  The product with the reciprocal
+// is within 3 2^-24 |q| <= 2.3e-5 of that quotient, so it rounds to the same integer unless it is nearer than that to a tie;
+// then (one group of 512 values in 60) the quotients are taken in binary64.  That is exact: the product with the binary64
+// reciprocal is within 2^-52 of x / s, relatively, and a quotient of an 11-bit and a 24-bit number is never half way between
+// two binary32 numbers (25 bits) nor nearer to that than 2^-49, so rounding the product rounds the quotient.
+struct Coder {
+  float scale, inverse;
+  __device__ explicit Coder(float s) : scale(s), inverse(s > 0.f && s < __builtin_inff() ? 1.f / s : 0.f) {}
+  __device__ uint2_t operator()(half8_t x) const {
+    uint2_t word = {0x80808080u, 0x80808080u};
+    if (inverse == 0.f) return word;  // a block of zeros, or one that is not finite (its scale says so)
+    float q[8], off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = (float)x[i] * inverse;
+      q[i] = rintf(t);
+      off = fmaxf(off, fabsf(t - q[i]));
+    }
+    if (off > 0.49997f) {
+      const double exact = 1. / (double)scale;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = rintf((float)((double)x[i] * exact));
+    }
+    word = uint2_t{0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[i / 4] = __builtin_amdgcn_cvt_pk_u8_f32(q[i] + 128.f, i % 4, word[i / 4]);
+    return word;
+  }
+};
+
+__device__ __forceinline__ uint32_t scaled_down(uint32_t word, float by) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r = __builtin_amdgcn_cvt_pk_u8_f32(rintf((float)((int)(word >> 8 * j & 255) - 128) * by) + 128.f, j, r);
+  return r;
 }
 
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs a) {
-  __shared__ uint32_t words[kMaxDim * 16];  // value codes transposed: [dim][token quad], columns of 8 dims swizzled
-  __shared__ uint32_t wave_max[kThreads / 64];
-  const int tid = threadIdx.x, h = blockIdx.y;
-  const bool values = blockIdx.z != 0;
-  Place p;
-  if (!find_place(a.cache, a.batch, blockIdx.x, p)) return;
-  const int dim = a.cache.dim, columns = dim / 8;
-  const int64_t place = (int64_t)p.id * a.cache.heads + h;
-  const half_t *x = (values ? a.x[1] : a.x[0]) + h * (values ? a.head[1] : a.head[0]);
-  const int64_t stride = values ? a.token[1] : a.token[0];
-  const int rotary_dim = values || !a.turns ? 0 : a.rotary_dim;
+__device__ __forceinline__ uint32_t magnitudes(half8_t v, uint32_t most) {
+  const uint4_t bits = __builtin_bit_cast(uint4_t, v) & 0x7fff7fffu;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t two = bits[j], had = most;  // (a bit cast of the vector's element itself takes element 0)
+    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, two), __builtin_bit_cast(ushort2_t, had)));
+  }
+  return most;
+}
 
-  // the pieces: token quad q (slots 4q ... 4q+3), column c (dims 8c ... 8c+7); the largest magnitude as bits, where NaN > inf
-  half8_t piece[kPieces][4];
-  uint32_t most = 0;
+// kSize threads: one wave where blocks get few tokens, four otherwise
+template <int kSize>
+__global__ __launch_bounds__(kSize) void kv_append_kernel(AppendArgs a) {
+  constexpr int kAhead = 4;
+  extern __shared__ uint4_t append_shared[];  // rows: binary16 [token][dim]; turn: cosine and sine [token][pair]
+  __shared__ uint32_t wave_max[2][kSize / 64];
+  const int tid = threadIdx.x;
+  const bool values = blockIdx.y + a.first != 0;
+  // (heads run fastest: the workgroups under way together then cover whole rows of the tokens, not one head's stretch of each)
+  const int dim = a.cache.dim, columns = dim / 8, heads = a.cache.heads, groups = (heads + a.heads_per_group - 1) / a.heads_per_group;
+  Place p;
+  if (!find_place(a.cache, a.batch, blockIdx.x / groups, p)) return;
+  const int rotary_dim = values || !a.turns ? 0 : a.rotary_dim, pairs = rotary_dim / 2;
+  const half_t *from = (values ? a.x[1] : a.x[0]) + p.row * (values ? a.token[1] : a.token[0]);
+  const int64_t stride = values ? a.token[1] : a.token[0], head_stride = values ? a.head[1] : a.head[0];
+  half_t *rows = (half_t *)append_shared;
+  float2 *turn = (float2 *)(rows + p.count * dim);
+  const int twos = a.half_layout ? pairs / 8 : 0, per_token = columns - twos;  // (half layout: units of two pieces)
+  const int end = p.slot + p.count, units = p.count * per_token;
+  // n / columns = n * per_column >> 16 for n < 2048 and columns <= 32, likewise for units
+  const uint32_t per_column = (65536 + columns - 1) / columns, per_unit = (65536 + per_token - 1) / per_token;
+  // a unit's pairs lie apart, pair j of unit u at j * stretch + u: neighbouring threads read neighbouring angles
+  const int per = a.half_layout ? 8 : 4, stretch = pairs / per;
+  if (pairs > 0) {  // (a thread keeps its pair, where it would wait for another one's turns with every angle)
+    const int together = max(kSize / pairs, 1);
+    for (int i = tid % pairs; i < pairs; i += kSize) {
+      const double turns = a.turns[i];
+      const int at = i % per * stretch + i / per;
+      for (int token = tid / pairs; token < p.count && tid < together * pairs; token += together)
+        turn[token * pairs + at] = rotary_turn(p.position + token, turns, a.factor, false);
+    }
+  }
+
+  const int h0 = blockIdx.x % groups * a.heads_per_group, h1 = min(heads, h0 + a.heads_per_group);
+  for (int h = h0; h < h1; ++h) {
+    const int64_t place = (int64_t)p.id * heads + h;
+    const half_t *x = from + h * head_stride;
+    float *scale_at = (values ? a.cache.v_scale : a.cache.k_scale) + place;
+    const float old = p.slot > 0 ? *scale_at : 0.f;
+    if (rotary_dim > 0 && h == h0) __syncthreads();  // (the angles are there)
+    uint32_t most = 0;  // the largest magnitudes, as two 16-bit patterns: NaN above infinity above all numbers
+    const auto put = [&](int token, int d, half8_t w) {
+      most = magnitudes(w, most);
+      *(half8_t *)(rows + token * dim + d) = w;
+    };
+    for (int n0 = tid; n0 < units; n0 += kAhead * kSize) {
+      half8_t v[kAhead], other[kAhead];
 #pragma unroll
-  for (int n = 0; n < kPieces; ++n) {
-    const int q = (tid + n * kThreads) / columns, c = (tid + n * kThreads) % columns;
+      for (int i = 0; i < kAhead; ++i) {
+        const int n = n0 + i * kSize, token = n * per_unit >> 16, u = n - token * per_token;
+        v[i] = other[i] = half8_t{};
+        if (n >= units) continue;
+        // a unit is 8 dims, or, among the first of a token, 8 dims and those they are turned with
+        v[i] = *(const half8_t *)(x + token * stride + (u < twos ? u : u + twos) * 8);
+        if (u < twos) other[i] = *(const half8_t *)(x + token * stride + pairs + u * 8);
+      }
+#pragma unroll 1
+      for (int i = 0; i < kAhead; ++i) {
+        const int n = n0 + i * kSize, token = n * per_unit >> 16, u = n - token * per_token;
+        if (n >= units) break;
+        half8_t w = v[0];
+        if (u < twos) {
+          half8_t w2;
+          const float2 *cs = turn + token * pairs + u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int token = 4 * q + i - p.slot;
-      half8_t v = {};
-      if (q < 16 && token >= 0 && token < p.count) {
-        const half_t *row = x + (p.row + token) * stride;
-        v = *(const half8_t *)(row + c * 8);
-        if (c * 8 < rotary_dim) {
-          const int position = p.position + token;
-          if (a.half_layout) {
-            const int pairs = rotary_dim / 2, at = c * 8 < pairs ? c * 8 : c * 8 - pairs;
-            const half8_t other = *(const half8_t *)(row + (c * 8 < pairs ? c * 8 + pairs : at));
+          for (int j = 0; j < 8; ++j) {
+            half_t lo, hi;
+            rotary_pair((float)w[j], (float)other[0][j], cs[j * stretch], lo, hi);
+            w[j] = lo, w2[j] = hi;
+          }
+          put(token, pairs + u * 8, w2);
+        } else if (twos == 0 && u * 8 < rotary_dim) {
+          const float2 *cs = turn + token * pairs + u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float2 cs = rotary_turn(position, a.turns[at + j], a.factor, false);
-              half_t lo, hi;
-              if (c * 8 < pairs)
-                rotary_pair((float)v[j], (float)other[j], cs, lo, hi);
-              else
-                rotary_pair((float)other[j], (float)v[j], cs, lo, hi);
-              v[j] = c * 8 < pairs ? lo : hi;
-            }
-          } else {
+          for (int j = 0; j < 4; ++j) {
+            half_t lo, hi;
+            rotary_pair((float)w[2 * j], (float)w[2 * j + 1], cs[j * stretch], lo, hi);
+            w[2 * j] = lo, w[2 * j + 1] = hi;
+          }
+        }
+        put(token, (u < twos ? u : u + twos) * 8, w);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 cs = rotary_turn(position, a.turns[c * 4 + j], a.factor, false);
-              half_t lo, hi;
-              rotary_pair((float)v[2 * j], (float)v[2 * j + 1], cs, lo, hi);
-              v[2 * j] = lo, v[2 * j + 1] = hi;
-            }
+        for (int k = 0; k + 1 < kAhead; ++k) v[k] = v[k + 1], other[k] = other[k + 1];  // (one copy of this code for the four)
+      }
+    }
+    most = max(most & 0xffff, most >> 16);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    if ((tid & 63) == 0) wave_max[h & 1][tid >> 6] = most;
+    __syncthreads();  // (every thread has read the old scale, too)
+#pragma unroll
+    for (int w = 0; w < kSize / 64; ++w) most = max(most, wave_max[h & 1][w]);
+    const float need = (float)__builtin_bit_cast(half_t, (uint16_t)most) / 127.f;  // infinite or NaN where an input is
+    float scale = old, shrink = 1.f;
+    if (!(need <= old) && old == old) {  // (a scale that is NaN stays)
+      scale = need;
+      if (old > 0.f && need < __builtin_inff()) {
+        int e;
+        if (frexpf(need / old, &e) == 0.5f) --e;
+        scale = ldexpf(old, e);
+        shrink = ldexpf(1.f, -e);
+      }
+    }
+    if (tid == 0 && (scale != old || p.slot == 0)) *scale_at = scale;
+
+    uint8_t *codes = (values ? a.cache.v_codes : a.cache.k_codes) + place * kBlock * dim;
+    if (shrink != 1.f) {  // tokens that were there: slots [0, slot)
+      for (int n = tid; n < (values ? dim * 16 : p.slot * dim / 4); n += kSize) {
+        const int t0 = values ? n % 16 * 4 : 0;
+        if (values && t0 >= p.slot) continue;
+        const uint32_t w = ((uint32_t *)codes)[n], keep = values && t0 + 4 > p.slot ? 0xffffffffu << 8 * (p.slot - t0) : 0u;
+        ((uint32_t *)codes)[n] = (scaled_down(w, shrink) & ~keep) | (w & keep);
+      }
+      if (values) __syncthreads();  // (a word may hold bytes of new tokens too, stored below)
+    }
+
+    const Coder code(scale);
+    if (!values || p.count < kFew) {
+#pragma unroll 2
+      for (int n = tid; n < p.count * columns; n += kSize) {
+        const int token = n * per_column >> 16, c = n - token * columns;
+        const half8_t v = *(const half8_t *)(rows + token * dim + c * 8);
+        const uint2_t w = code(v);
+        if (!values) {
+          *(uint2_t *)(codes + (p.slot + token) * dim + c * 8) = w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) codes[(c * 8 + j) * kBlock + p.slot + token] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+        }
+      }
+    } else {
+      for (int n = tid; n < dim * 2; n += kSize) {  // two dims, 16 slots
+        const int d = n / 4 * 2, t0 = n % 4 * 16;  // (a row's 64 bytes by four lanes)
+        if (t0 + 15 < p.slot || t0 >= end) continue;
+        const half_t *column = rows + (t0 - p.slot) * dim + d;
+        uint4_t w[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {  // 8 slots
+          half8_t v[2];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const half2_t two = *(const half2_t *)(column + (min(max(t0 + 8 * q + i, p.slot), end - 1) - t0) * dim);
+            v[0][i] = two[0], v[1][i] = two[1];
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint2_t eight = code(v[i]);
+            w[i][2 * q] = eight[0], w[i][2 * q + 1] = eight[1];
           }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, (uint32_t)(__builtin_bit_cast(uint16_t, (half_t)v[j]) & 0x7fff));
-      }
-      piece[n][i] = v;
-    }
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-  if ((tid & 63) == 0) wave_max[tid >> 6] = most;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) most = max(most, wave_max[w]);
-  const float need = (float)__builtin_bit_cast(half_t, (uint16_t)most) / 127.f;  // infinite or NaN where an input is
-
-  float *scale_at = (values ? a.cache.v_scale : a.cache.k_scale) + place;
-  const float old = p.slot > 0 ? *scale_at : 0.f;
-  float scale = old, shrink = 1.f;
-  if (!(need <= old) && old == old) {  // (a scale that is NaN stays)
-    scale = need;
-    if (old > 0.f && need < __builtin_inff()) {
-      int e;
-      if (frexpf(need / old, &e) == 0.5f) --e;
-      scale = ldexpf(old, e);
-      shrink = ldexpf(1.f, -e);
-    }
-  }
-  // (every thread has read the old scale before one replaces it)
-  __syncthreads();
-  if (tid == 0 && (scale != old || p.slot == 0)) *scale_at = scale;
-
-  uint8_t *codes = (values ? a.cache.v_codes : a.cache.k_codes) + place * kBlock * dim;
-  if (shrink != 1.f) {  // tokens that were there: slots [0, slot)
-    if (!values) {
-      for (int n = tid; n < p.slot * dim / 4; n += kThreads) {
-        uint32_t w = ((uint32_t *)codes)[n], r = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r |= (uint32_t)(int)(rintf((float)((int)(w >> 8 * j & 255) - 128) * shrink) + 128.f) << 8 * j;
-        ((uint32_t *)codes)[n] = r;
-      }
-    } else {
-      for (int n = tid; n < dim * 16; n += kThreads) {
-        const int t0 = n % 16 * 4;
-        if (t0 >= p.slot) continue;
-        uint32_t w = ((uint32_t *)codes)[n], r = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t byte = w >> 8 * j & 255;
-          r |= (t0 + j < p.slot ? (uint32_t)(int)(rintf((float)((int)byte - 128) * shrink) + 128.f) : byte) << 8 * j;
+        for (int i = 0; i < 2; ++i) {
+          uint8_t *to = codes + (d + i) * kBlock + t0;
+          if (t0 >= p.slot && t0 + 16 <= end) {
+            *(uint4_t *)to = w[i];
+          } else {
+            for (int j = max(p.slot - t0, 0); j < min(end - t0, 16); ++j) {
+              const uint32_t word = j < 4 ? w[i][0] : j < 8 ? w[i][1] : j < 12 ? w[i][2] : w[i][3];
+              to[j] = (uint8_t)(word >> 8 * (j & 3));
+            }
+          }
         }
-        ((uint32_t *)codes)[n] = r;
-      }
-      __syncthreads();  // (a word may hold bytes of new tokens too, stored below)
-    }
-  }
-
-  const int end = p.slot + p.count;
-  const bool few = p.count < 8;  // value codes of few tokens are stored byte by byte, each row of 64 tokens apart
-#pragma unroll
-  for (int n = 0; n < kPieces; ++n) {
-    const int q = (tid + n * kThreads) / columns, c = (tid + n * kThreads) % columns;
-    if (q >= 16 || 4 * q + 3 < p.slot || 4 * q >= end) continue;
-    if (!values) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int slot = 4 * q + i;
-        if (slot < p.slot || slot >= end) continue;
-        uint2_t w = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j / 4] |= quantise(piece[n][i][j], scale) << 8 * (j % 4);
-        *(uint2_t *)(codes + slot * dim + c * 8) = w;
-      }
-    } else if (few) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int slot = 4 * q + i;
-        if (slot < p.slot || slot >= end) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) codes[(c * 8 + j) * kBlock + slot] = (uint8_t)quantise(piece[n][i][j], scale);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= quantise(piece[n][i][j], scale) << 8 * i;
-        words[(c * 8 + j) * 16 + (q ^ (c & 15))] = w;
       }
     }
-  }
-  if (values && !few) {
-    __syncthreads();
-    for (int n = tid; n < dim * 4; n += kThreads) {
-      const int d = n / 4, q0 = n % 4 * 4, t0 = q0 * 4;
-      if (t0 + 15 < p.slot || t0 >= end) continue;
-      uint4_t w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = words[d * 16 + ((q0 + j) ^ (d / 8 & 15))];
-      uint8_t *to = codes + d * kBlock + t0;
-      if (t0 >= p.slot && t0 + 16 <= end) {
-        *(uint4_t *)to = w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (t0 + j >= p.slot && t0 + j < end) to[j] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
-      }
-    }
+    __syncthreads();  // (the next head's rows)
   }
 }
 
@@ -229,10 +282,10 @@ struct GatherArgs {
 
 // The values of a batch's new tokens as binary16, [tokens][heads][dim]: one rounding of code * scale.
 __global__ __launch_bounds__(kThreads) void kv_gather_kernel(GatherArgs a) {
-  const int tid = threadIdx.x, h = blockIdx.y;
-  const bool values = blockIdx.z != 0;
+  const int tid = threadIdx.x, h = blockIdx.x % a.cache.heads;
+  const bool values = blockIdx.y != 0;
   Place p;
-  if (!find_place(a.cache, a.batch, blockIdx.x, p)) return;
+  if (!find_place(a.cache, a.batch, blockIdx.x / a.cache.heads, p)) return;
   const int dim = a.cache.dim, columns = dim / 8;
   const int64_t place = (int64_t)p.id * a.cache.heads + h;
   const float scale = (values ? a.cache.v_scale : a.cache.k_scale)[place];
@@ -272,13 +325,24 @@ __global__ __launch_bounds__(kThreads) void kv_gather_kernel(GatherArgs a) {
   }
 }
 
+// A kernel has to be told of more than 64 KiB of LDS, on each device.
+int allow_lds(const void *kernel, size_t bytes) {
+  if (bytes <= 63 << 10) return GQ_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? GQ_OK : fail((int)e, "kv_append_kernel: %s", hipGetErrorString(e));
+}
+
 // (sequence, block) pairs at most: a sequence of n new tokens reaches into (n + 62) / 64 + 1 blocks
-unsigned most_places(const KvBatch &b) { return (unsigned)(b.tokens / kBlock + 2 * b.sequences); }
+int64_t most_places(const KvBatch &b) { return b.tokens / kBlock + 2 * (int64_t)b.sequences; }
+
+// 2^24 rows and 2^20 sequences of 1024 heads would be more workgroups than a grid has
+bool too_many(const KvCache &cache, const KvBatch &batch) { return most_places(batch) * cache.heads > 0x7fffffff / kThreads; }
 
 }  // namespace
 
 int launch_kv_append(const KvCache &cache, const KvBatch &batch, const uint16_t *k, int64_t k_token, int64_t k_head,
                      const uint16_t *v, int64_t v_token, int64_t v_head, const gq_rotary *rotary, hipStream_t stream) {
+  if (too_many(cache, batch)) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_append_f16: too many rows, sequences and heads for one launch");
   AppendArgs a = {};
   a.cache = cache, a.batch = batch;
   a.x[0] = (const half_t *)k, a.token[0] = k_token, a.head[0] = k_head;
@@ -287,13 +351,30 @@ int launch_kv_append(const KvCache &cache, const KvBatch &batch, const uint16_t 
     a.turns = rotary->turns, a.factor = rotary->factor, a.rotary_dim = rotary->rotary_dim;
     a.half_layout = rotary->layout == GQ_ROTARY_HALF;
   }
-  kv_append_kernel<<<dim3(most_places(batch), cache.heads, 2), kThreads, 0, stream>>>(a);
+  const int64_t places = most_places(batch);
+  const int rows = batch.tokens < kBlock ? batch.tokens : kBlock;
+  const size_t codes = (size_t)rows * cache.dim * sizeof(half_t), angles = rotary ? (size_t)rows * rotary->rotary_dim / 2 * sizeof(float2) : 0;
+  if (batch.tokens < kFew * batch.sequences) {
+    a.heads_per_group = 1;
+    if (const int rc = allow_lds((const void *)kv_append_kernel<64>, codes + angles)) return rc;
+    kv_append_kernel<64><<<dim3((unsigned)(places * cache.heads), 2), 64, codes + angles, stream>>>(a);
+  } else {
+    // Keys and values apart: the angles take as much LDS as the rows or twice that, which only the keys' workgroups need.  They
+    // are worth sharing between heads where there are workgroups enough anyway, as is what every workgroup does first.
+    if (const int rc = allow_lds((const void *)kv_append_kernel<kThreads>, codes + angles)) return rc;
+    a.heads_per_group = places * cache.heads >= 1536 ? 4 : 1;
+    const int groups = (cache.heads + a.heads_per_group - 1) / a.heads_per_group;
+    kv_append_kernel<kThreads><<<(unsigned)(places * groups), kThreads, codes + angles, stream>>>(a);
+    a.first = 1;
+    kv_append_kernel<kThreads><<<(unsigned)(places * groups), kThreads, codes, stream>>>(a);
+  }
   return check_launch("kv_append_kernel");
 }
 
 int launch_kv_gather(const KvCache &cache, const KvBatch &batch, uint16_t *k, uint16_t *v, hipStream_t stream) {
+  if (too_many(cache, batch)) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_gather_f16: too many rows, sequences and heads for one launch");
   GatherArgs a = {cache, batch, {(half_t *)k, (half_t *)v}};
-  kv_gather_kernel<<<dim3(most_places(batch), cache.heads, 2), kThreads, 0, stream>>>(a);
+  kv_gather_kernel<<<dim3((unsigned)(most_places(batch) * cache.heads), 2), kThreads, 0, stream>>>(a);
   return check_launch("kv_gather_kernel");
 }
 

@@ -4,8 +4,7 @@
 //   out = (a c - b s, a s + b c) with (c, s) = factor * (cos, sin)(2 pi p turns[i]), dims behind r copied.
 //
 // Bound by HBM: 4 bytes an element and little arithmetic.  A workgroup takes one token and some of its heads: the r/2
-// angles are formed once in LDS and serve all of these heads (binary64 phase, sincospif: about 60 instructions a pair,
-// which per head and pair would cost as much as the memory traffic).
+// angles are formed once in LDS and serve all of these heads.
 #include "gq_rotary.h"
 
 namespace gq {
