@@ -219,20 +219,19 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) acc[r][t] = float4_t{};
-  // 64 features a step: a lane has 16 consecutive ones of a row (both operands agree on which), so that a row's 128 bytes are
-  // asked for together
+  // 64 features a step, so that a row's 128 bytes are asked for together
   half8_t xf[2][kTiles][2], wf[2][kRankTiles][2];
   const auto load = [&](int set, int64_t k) {
-    k += g * 16;
+    k += g * 8;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) xf[set][t][u] = load8<kWide>(x[t] + k + 8 * u, to - k - 8 * u);
+      for (int u = 0; u < 2; ++u) xf[set][t][u] = load8<kWide>(x[t] + k + 32 * u, to - k - 32 * u);
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (r * 16 < a.rank) wf[set][r][u] = load8_any<kWide>(wr[r], k + 8 * u, a.features);
+        if (r * 16 < a.rank) wf[set][r][u] = load8_any<kWide>(wr[r], k + 32 * u, a.features);
   };
   const auto multiply = [&](int set) {
 #pragma unroll
@@ -245,12 +244,21 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
           acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[set][r][u], xf[set][t][u], acc[r][t], 0, 0, 0);
       }
   };
-  if (from < to) load(0, from);
-  for (int64_t k = from; k < to; k += 128) {
-    if (k + 64 < to) load(1, k + 64);
+  // Tiles start at different places of their range: rows are often a power of two apart, and tiles that walked their columns in
+  // step would keep asking the same few memory channels (8192 rows of 16384: 87 us, 74 us so).
+  const int steps = (int)((to - from + 63) / 64);
+  int step = steps > 0 ? blockIdx.x * 5 % steps : 0;
+  const auto next = [&] {
+    const int64_t k = from + 64 * step;
+    step = step + 1 < steps ? step + 1 : 0;
+    return k;
+  };
+  if (steps > 0) load(0, next());
+  for (int i = 0; i < steps; i += 2) {
+    if (i + 1 < steps) load(1, next());
     multiply(0);
-    if (k + 64 >= to) break;
-    if (k + 128 < to) load(0, k + 128);
+    if (i + 1 >= steps) break;
+    if (i + 2 < steps) load(0, next());
     multiply(1);
   }
   // sum of the four waves, 16 rows at a time: [waves][16 rows][kRank + 4]
@@ -347,8 +355,8 @@ __device__ __forceinline__ float4_t sum_of_splits(const float *p, int64_t stride
 }
 
 // The workgroup sums its rows' v over the splits into LDS, where its waves take their operands from.  Then wave w takes 64
-// features at a time: row 4 g' + i of operand tile f is feature 16 g' + 4 f + i, so that a lane ends with 16 consecutive
-// features of one row (two 16-byte loads and stores, 128 bytes a row for the wave).  The weights and y of the next
+// features at a time: row 4 g' + i of operand tile f is feature 32 (f / 2) + 8 g' + 4 (f % 2) + i, so that a lane ends with 8
+// consecutive features of one row in each half (16-byte loads and stores, 64 bytes of a row together).  The weights and y of the next
 // piece are loaded before and among this one's products.
 template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
@@ -368,7 +376,7 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   const auto load_weights = [&](int set, int64_t n0) {
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-      const half_t *p = w + min(n0 + 16 * (m >> 2) + 4 * f + (m & 3), a.features - 1) * a.rank;
+      const half_t *p = w + min(n0 + 32 * (f >> 1) + 8 * (m >> 2) + 4 * (f & 1) + (m & 3), a.features - 1) * a.rank;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
         if (c * 32 < a.rank) wf[set][f][c] = load8_any<kWide>(p, c * 32 + g * 8, a.rank);
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   const auto load_y = [&](int t, int64_t n0) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int64_t n = n0 + 16 * g + 8 * half;
+      const int64_t n = n0 + 32 * half + 8 * g;
       y[t][half] = half8_t{};
       if (a.y) y[t][half] = load8<kWide>(a.y + row[t] * a.y_stride + n, to - n);
     }
@@ -442,11 +450,11 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
       const bool there = t * 16 + m < tile.count;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int64_t n = n0 + 16 * g + 8 * half;
+        const int64_t n = n0 + 32 * half + 8 * g;
         half8_t r;
         float sum[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // (tile f, row 4 g + i of the accumulators is feature 16 g + 4 f + i)
+        for (int j = 0; j < 8; ++j)  // (tile 2 half + j / 4, row 4 g + j % 4 of the accumulators)
           sum[j] = (float)y[t][half][j] + acc[2 * half + j / 4][j % 4];
         activate(sum, a.act);
 #pragma unroll
