@@ -202,7 +202,7 @@ template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_down_kernel(DownArgs a) {
   constexpr int kRankTiles = kRank / 16;
   extern __shared__ float shared[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   if ((int)blockIdx.x >= *a.tile_count) return;
   const AdapterTile tile = a.tiles[blockIdx.x];
   if (tile.adapter < 0) return;
@@ -219,21 +219,30 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) acc[r][t] = float4_t{};
-  // 64 features a step, so that a row's 128 bytes are asked for together
+  // 64 features a step, so that a row's 128 bytes are asked for together.  Loads are made without conditions (of other
+  // values of the row where it ends): a register that a load fills on one path only is copied, and the copy waits for it.
   half8_t xf[2][kTiles][2], wf[2][kRankTiles][2];
   const auto load = [&](int set, int64_t k) {
     k += g * 8;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) xf[set][t][u] = load8<kWide>(x[t] + k + 32 * u, to - k - 32 * u);
+      for (int u = 0; u < 2; ++u) xf[set][t][u] = load8_any<kWide>(x[t], k + 32 * u, a.features);
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (r * 16 < a.rank) wf[set][r][u] = load8_any<kWide>(wr[r], k + 32 * u, a.features);
+      for (int u = 0; u < 2; ++u) wf[set][r][u] = load8_any<kWide>(wr[r], k + 32 * u, a.features);
   };
-  const auto multiply = [&](int set) {
+  const auto multiply = [&](int set, int64_t k) {
+    if (k + 64 > to) {  // values behind the range are zeros
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (k + 32 * u + g * 8 + j >= to) xf[set][t][u][j] = (half_t)0.f;
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -246,20 +255,19 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   };
   // Tiles start at different places of their range: rows are often a power of two apart, and tiles that walked their columns in
   // step would keep asking the same few memory channels (8192 rows of 16384: 87 us, 74 us so).
-  const int steps = (int)((to - from + 63) / 64);
-  int step = steps > 0 ? blockIdx.x * 5 % steps : 0;
-  const auto next = [&] {
-    const int64_t k = from + 64 * step;
-    step = step + 1 < steps ? step + 1 : 0;
-    return k;
+  const int steps = (int)((to - from + 63) / 64), turn = steps > 0 ? blockIdx.x * 5 % steps : 0;
+  const auto place = [&](int i) {
+    const int at = turn + min(i, steps - 1);
+    return from + 64 * (int64_t)(at < steps ? at : at - steps);
   };
-  if (steps > 0) load(0, next());
-  for (int i = 0; i < steps; i += 2) {
-    if (i + 1 < steps) load(1, next());
-    multiply(0);
-    if (i + 1 >= steps) break;
-    if (i + 2 < steps) load(0, next());
-    multiply(1);
+  if (steps > 0) {
+    load(0, place(0));
+    for (int i = 0; i < steps; i += 2) {
+      load(1, place(i + 1));
+      multiply(0, place(i));
+      load(0, place(i + 2));
+      if (i + 1 < steps) multiply(1, place(i + 1));
+    }
   }
   // sum of the four waves, 16 rows at a time: [waves][16 rows][kRank + 4]
   float *v = a.v + ((int64_t)blockIdx.y * a.rows + tile.begin) * kRank;
@@ -299,9 +307,10 @@ struct UpArgs {
   const float *v;   // [splits][rows][kRank]
   const half_t *w;  // [adapters][features][rank]
   const float *scaling;
-  const half_t *y;  // NULL: zeros
+  const half_t *y;  // out where there is none
   half_t *out;
   int64_t y_stride, out_stride;
+  bool has_y;
   const AdapterTile *tiles;
   const int *tile_count, *order;
   int64_t rows, features, range;  // features of one workgroup, a multiple of 256
@@ -362,7 +371,7 @@ template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
   constexpr int kChunks = kRank / 32, kRow = kRank + 4;
   __shared__ float v[kTiles * 16 * kRow];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   if ((int)blockIdx.x >= *a.tile_count) return;
   const AdapterTile tile = a.tiles[blockIdx.x];
   const bool with = tile.adapter >= 0;
@@ -370,6 +379,13 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   const half_t *w = a.w + (int64_t)max(tile.adapter, 0) * a.rank * a.features;
   const float scaling = with ? a.scaling[tile.adapter] : 0.f;
   const int64_t from = blockIdx.y * a.range, to = min(a.features, from + a.range), first = from + wave * 64;
+  // (tiles start at different pieces of the range and loads have no conditions, as in adapter_down_kernel)
+  const int pieces = first < to ? (int)((to - first + kWaves * 64 - 1) / (kWaves * 64)) : 0, turn = pieces > 0 ? blockIdx.x * 5 % pieces : 0;
+  const auto place = [&](int i) {
+    if (pieces == 0) return (int64_t)0;  // (a wave without features still loads, and drops, the first ones)
+    const int at = turn + min(i, pieces - 1);
+    return first + (int64_t)(at < pieces ? at : at - pieces) * (kWaves * 64);
+  };
 
   half8_t wf[2][4][kChunks], y[kTiles][2];
   int64_t row[kTiles];
@@ -379,25 +395,24 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
       const half_t *p = w + min(n0 + 32 * (f >> 1) + 8 * (m >> 2) + 4 * (f & 1) + (m & 3), a.features - 1) * a.rank;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
-        if (c * 32 < a.rank) wf[set][f][c] = load8_any<kWide>(p, c * 32 + g * 8, a.rank);
+        wf[set][f][c] = load8_any<kWide>(p, c * 32 + g * 8, a.rank);
     }
   };
   const auto load_y = [&](int t, int64_t n0) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int64_t n = n0 + 32 * half + 8 * g;
-      y[t][half] = half8_t{};
-      if (a.y) y[t][half] = load8<kWide>(a.y + row[t] * a.y_stride + n, to - n);
+      y[t][half] = load8_any<kWide>(a.y + row[t] * a.y_stride, n, a.features);
     }
   };
-  if (with && first < to) load_weights(0, first);
+  load_weights(0, place(0));
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) row[t] = a.order[tile.begin + min(t * 16 + m, tile.count - 1)];
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) load_y(t, first);
+  for (int t = 0; t < kTiles; ++t) load_y(t, place(0));
 
-  half8_t hi[kTiles][kChunks], lo[kTiles][kChunks];
-  float back[kTiles];
+  half8_t hi[kTiles][kChunks] = {}, lo[kTiles][kChunks] = {};
+  float back[kTiles] = {};
   if (with) {
     for (int n = threadIdx.x; n < tile.count * (kRank / 4); n += kThreads) {
       const int i = n / (kRank / 4), r = n % (kRank / 4) * 4;
@@ -427,9 +442,8 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
     }
   }
 
-  const auto piece = [&](int set, int64_t n0) {
-    const int64_t next = n0 + kWaves * 64;
-    if (with && next < to) load_weights(set ^ 1, next);
+  const auto piece = [&](int set, int64_t n0, int64_t next) {
+    load_weights(set ^ 1, next);
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       float4_t acc[4];
@@ -447,33 +461,36 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[f] *= back[t];
       }
-      const bool there = t * 16 + m < tile.count;
+      half8_t r[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int64_t n = n0 + 32 * half + 8 * g;
-        half8_t r;
         float sum[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)  // (tile 2 half + j / 4, row 4 g + j % 4 of the accumulators)
-          sum[j] = (float)y[t][half][j] + acc[2 * half + j / 4][j % 4];
+          sum[j] = (a.has_y ? (float)y[t][half][j] : 0.f) + acc[2 * half + j / 4][j % 4];
         activate(sum, a.act);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = (half_t)sum[j];
+        for (int j = 0; j < 8; ++j) r[half][j] = (half_t)sum[j];
+      }
+      load_y(t, next);
+      if (t * 16 + m >= tile.count) continue;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int64_t n = n0 + 32 * half + 8 * g;
         half_t *o = a.out + row[t] * a.out_stride + n;
         if (kWide) {
-          if (there && n < to) *(half8_t *)o = r;
+          if (n < to) *(half8_t *)o = r[half];
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (there && n + j < to) o[j] = r[j];
+            if (n + j < to) o[j] = r[half][j];
         }
       }
-      if (next < to) load_y(t, next);
     }
   };
-  for (int64_t n0 = first; n0 < to; n0 += 2 * kWaves * 64) {
-    piece(0, n0);
-    if (n0 + kWaves * 64 < to) piece(1, n0 + kWaves * 64);
+  for (int i = 0; i < pieces; i += 2) {
+    piece(0, place(i), place(i + 1));
+    if (i + 1 < pieces) piece(1, place(i + 1), place(i + 2));
   }
 }
 
@@ -598,7 +615,7 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
   __shared__ float shared[kWaves * 16 * kRow];  // at first the segment's rows
   int *order = (int *)shared;
   static_assert(sizeof(shared) >= kAdapterSegment * sizeof(int), "a segment's rows fit");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const bool second = blockIdx.z & 1;
   const int rank0 = (blockIdx.z >> 1) * 64;
   const OuterSide &side = second ? a.side[1] : a.side[0];
@@ -614,6 +631,8 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
   for (int r = 0; r < kRankTiles; ++r)
 #pragma unroll
     for (int c = 0; c < 8; ++c) acc[r][c] = float4_t{};
+  // Loads are made without conditions (of the last rows and operands again where there are no more), for a register that a load
+  // fills on one path only is copied, and the copy waits for it.
   half8_t x[2][8], h[2][kRankTiles], l[2][kRankTiles];
   const auto load = [&](int set, int i0) {
 #pragma unroll
@@ -624,7 +643,7 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
     }
   };
   const auto load_operand = [&](int set, int i0) {
-    const half_t *at = hi + (int64_t)(rank0 + m) * kAdapterSegment + i0 + g * 8;
+    const half_t *at = hi + (int64_t)(rank0 + m) * kAdapterSegment + min(i0, kAdapterSegment - 32) + g * 8;
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) {
       h[set][r] = *(const half8_t *)(at + r * 16 * kAdapterSegment);
@@ -639,8 +658,9 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
 #pragma unroll
       for (int j = 0; j < 8; ++j) xf[c][j] = x[set][j][c];
     // (the operand first: loads arrive in order, and it is needed a step before these rows)
-    if (i0 + kStep < seg.count) load_operand(set ^ 1, i0 + kStep);
-    if (i0 + 2 * kStep < seg.count) load(set, i0 + 2 * kStep);
+    load_operand(set ^ 1, i0 + kStep);
+    load(set, i0 + 2 * kStep);
+    if (i0 >= seg.count) return;
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) {
       if (rank0 + r * 16 >= a.rank) continue;
@@ -651,11 +671,12 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
     }
   };
   const int start = wave * 32;
-  if (start < seg.count) load(0, start), load_operand(0, start);
-  if (start + kStep < seg.count) load(1, start + kStep);
+  load_operand(0, start);
+  load(0, start);
+  load(1, start + kStep);
   for (int i0 = start; i0 < seg.count; i0 += 2 * kStep) {
     multiply(0, i0);
-    if (i0 + kStep < seg.count) multiply(1, i0 + kStep);
+    multiply(1, i0 + kStep);
   }
   const float back = side.back[blockIdx.x];
   const int64_t f0 = (int64_t)blockIdx.y * 128;
@@ -767,7 +788,8 @@ int launch_down(const Batch &b, const half_t *x, int64_t x_stride, const half_t 
 int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, const float *scaling, const half_t *y, int64_t y_stride,
               half_t *out, int64_t out_stride, int64_t features, int64_t rank, int act, hipStream_t stream) {
   UpArgs a;
-  a.v = v, a.w = w, a.scaling = scaling, a.y = y, a.out = out, a.y_stride = y_stride, a.out_stride = out_stride;
+  a.v = v, a.w = w, a.scaling = scaling, a.has_y = y != nullptr, a.out = out, a.out_stride = out_stride;
+  a.y = y ? y : out, a.y_stride = y ? y_stride : out_stride;
   a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0), a.order = b.words + b.plan.order;
   a.rows = b.plan.rows, a.features = features, a.rank = (int)rank, a.splits = (int)splits, a.act = act;
   a.skip_rows_without = y == out && y_stride == out_stride && act == GQ_ACT_NONE;
