@@ -546,7 +546,7 @@ struct OuterSide {
   const float *v;     // [splits][rows][kRank]
   const float *most;  // [splits][tiles]
   int splits;
-  half_t *operand;  // [segments][hi, lo][kRank][kAdapterSegment]
+  half_t *operand;  // [segments][steps of 32 rows][hi, lo][16 ranks][lane][8]: 1 KiB for a wave's load
   float *back;      // [segments]
   float *grad;      // [adapters][rank][features], turned: [adapters][features][rank]
   float *parts;     // [parts], the same
@@ -597,10 +597,10 @@ __global__ __launch_bounds__(kThreads) void adapter_operand_kernel(OuterArgs a) 
     }
   }
   __syncthreads();
-  half_t *to = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment;
-  for (int n = tid; n < 2 * kRank * 8; n += kThreads) {
-    const int which = n / (kRank * 8), r = n / 8 % kRank, i = n % 8 * 8;
-    *(half8_t *)(to + (int64_t)(which * kRank + r) * kAdapterSegment + i0 + i) = *(const half8_t *)&piece[which][r][i];
+  half_t *to = side.operand + ((int64_t)blockIdx.x * kAdapterSegment + i0) * 2 * kRank;
+  for (int n = tid; n < 2 * 2 * kRank * 4; n += kThreads) {
+    const int m = n % 16, g = n / 16 % 4, r = n / 64 % (kRank / 16), which = n / (kRank * 4) % 2, step = n / (kRank * 8);
+    *(half8_t *)(to + n * 8) = *(const half8_t *)&piece[which][r * 16 + m][step * 32 + g * 8];
   }
 }
 
@@ -623,7 +623,8 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
   const AdapterTile seg = a.segments[blockIdx.x];
   for (int n = threadIdx.x; n < seg.count; n += kThreads) order[n] = a.order[seg.begin + n];
   __syncthreads();
-  const half_t *hi = side.operand + (int64_t)blockIdx.x * 2 * kRank * kAdapterSegment;
+  // (in the order of the loads: rows of it a power of two apart would all be asked of one memory channel)
+  const half_t *operand = side.operand + (int64_t)blockIdx.x * kAdapterSegment * 2 * kRank + rank0 * 32 + lane * 8;
   const int64_t f = (int64_t)blockIdx.y * 128 + m * 8;
 
   float4_t acc[kRankTiles][8];
@@ -643,11 +644,11 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
     }
   };
   const auto load_operand = [&](int set, int i0) {
-    const half_t *at = hi + (int64_t)(rank0 + m) * kAdapterSegment + min(i0, kAdapterSegment - 32) + g * 8;
+    const half_t *at = operand + (int64_t)min(i0, kAdapterSegment - 32) * 2 * kRank;
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) {
-      h[set][r] = *(const half8_t *)(at + r * 16 * kAdapterSegment);
-      l[set][r] = *(const half8_t *)(at + (kRank + r * 16) * kAdapterSegment);
+      h[set][r] = *(const half8_t *)(at + r * 512);
+      l[set][r] = *(const half8_t *)(at + kRank * 32 + r * 512);
     }
   };
   constexpr int kStep = kWaves * 32;
