@@ -437,7 +437,7 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
 
 /*
  * 8-bit key/value cache in blocks of GQ_KV_BLOCK tokens, one binary32 scale for the keys and one for the values of each
- * (block, head); value = (byte - 128) * scale, bytes 1 ... 255.  head_dim is a multiple of 16, at most 256; the code arrays are
+ * (block, head); value = (byte - 128) * scale, bytes 1 ... 255, scales not negative.  head_dim is a multiple of 16, at most 256; the code arrays are
  * 16-byte aligned.
  *
  * A batch is B sequences.  Rows offsets[b] ... offsets[b + 1] - 1 of the row tensors (k, v, q, out) are the newest tokens of

@@ -23,8 +23,7 @@ namespace gq {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kRows = 16;
-constexpr int kMostGroups = 512;
-constexpr int kTileLeast = 64;
+constexpr int kMostGroups = 512, kTileRows = 128, kTileLeast = 64;
 
 struct AttentionArgs {
   KvCache cache;
@@ -34,8 +33,10 @@ struct AttentionArgs {
   int64_t q_token, q_head, o_token, o_head;
   int group;         // query heads of one kv head
   float scale_log2;  // softmax scale x log2(e)
-  float *parts;      // [2 groups of the grid][kRows][dim], then maxima and sums [2 groups][2][kRows]
-  int groups;
+  // kv_split_kernel: [2 groups][kRows][dim], then maxima and sums [2 groups][2][kRows] (groups: the grid's);
+  // kv_tile_kernel, where `splits` of them share a tile: [groups][splits][kTileRows][dim], then [groups][splits][2][kTileRows]
+  float *parts;
+  int groups, splits;
 };
 
 struct Shape {  // one sequence's share of the work
@@ -283,8 +284,11 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
 // Rescaling the accumulators for every block would cost as many vector instructions as the softmax.  The maximum in
 // use is only raised when scores pass it by more than 8 (probabilities up to 2^8 then), and the value scale enters the exponent
 // as its ratio to a reference, which only moves when the ratio leaves [1/16, 16]; the sum takes the ratio back out.
+//
+// A grid too small for the device is divided over the keys as well: `splits` workgroups share a tile and kv_tile_join_kernel adds
+// their parts, in their order.
 
-constexpr int kTileThreads = 256, kTileRows = 128;
+constexpr int kTileThreads = 256;
 
 __device__ __forceinline__ void store_codes(half_t *to, uint32_t lo, uint32_t hi) { *(half8_t *)to = eight_codes(lo, hi); }
 
@@ -329,7 +333,8 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
   const int wave_first = s.first + wave_row / a.group;                                          // its first row's position
   const int wave_last = wave_row < rows ? s.first + (min(wave_row + kRowsOfWave, rows) - 1) / a.group : -1;
   const int group_last = s.first + (min(row0 + kRowsOfGroup, rows) - 1) / a.group;
-  const int blocks = group_last < 0 ? 0 : group_last / kBlock + 1;
+  const int all_blocks = group_last < 0 ? 0 : group_last / kBlock + 1, share_of = (all_blocks + a.splits - 1) / a.splits;
+  const int first_block = min(all_blocks, (int)blockIdx.y * share_of), blocks = min(all_blocks, first_block + share_of);
 
   // staging: thread n has keys' piece (key, 16 dims c) and values' piece (dim d, 16 tokens)
   uint4_t raw_k[kPieces], raw_v[kPieces];
@@ -373,15 +378,18 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
   float reference = 1.f;
 #pragma unroll
   for (int i = 0; i < kDimTiles; ++i) o[i] = float16_t{};
-  if (blocks > 0) {
-    load(0);
-    if (there) stage(0);
+  if (first_block < blocks) {
+    load(first_block);
+    if (there) stage(first_block & 1);
   }
   bool fresh = true;
-  for (int block = 0; block < blocks; ++block) {
+  for (int block = first_block; block < blocks; ++block) {
     __syncthreads();
     const bool now = there;
-    const float key_scale = ks == 0.f ? 1.f : ks * fabsf(a.scale_log2), value_scale = vs;  // (keys of scale 0 are zeros)
+    // (not 0, which a masked score of -infinity would not survive: below 1e-30 every score is 0 to all that exp2 can tell)
+    float key_scale = ks * fabsf(a.scale_log2);
+    if (key_scale < 1e-30f) key_scale = 1e-30f;
+    const float value_scale = vs;
     if (block + 1 < blocks) load(block + 1);
     const int at = block * kBlock;
     if (now && at <= wave_last) {
@@ -444,33 +452,84 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
           pf[T][i >> 3][i & 7] = (half_t)p;
         }
       sum += part / share;
+      if (value_scale != 0.f) {  // (values of scale 0 are zeros, whatever their codes)
 #pragma unroll
-      for (int i = 0; i < kDimTiles; ++i)
+        for (int i = 0; i < kDimTiles; ++i)
 #pragma unroll
-        for (int T = 0; T < 2; ++T)
+          for (int T = 0; T < 2; ++T)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
-            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
-          }
+            for (int u = 0; u < 2; ++u) {
+              const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
+              o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
+            }
+      }
     }
     if (block + 1 < blocks && there) stage((block + 1) & 1);
   }
-  {
-    const float weight = sum + __shfl_xor(sum, 32);
-    const float factor = weight == 0.f ? 0.f : reference / weight;
-    const int row = row0 + wave * kRowsOfWave + m;
-    if (row >= rows) return;
-    half_t *to = a.out + (s.begin + row / a.group) * a.o_token + (int64_t)(h * a.group + row % a.group) * a.o_head;
+  const float weight = sum + __shfl_xor(sum, 32);
+  const int in_tile = wave * kRowsOfWave + m, row = row0 + in_tile;
+  if (row >= rows) return;
+  if (a.splits > 1) {
+    const int64_t slot = (int64_t)blockIdx.x * a.splits + blockIdx.y;
+    float *to = a.parts + (slot * kTileRows + in_tile) * dim, *stats = a.parts + (int64_t)a.groups * a.splits * kTileRows * dim + slot * 2 * kTileRows;
+    if (g == 0) stats[in_tile] = most, stats[kTileRows + in_tile] = weight;
 #pragma unroll
     for (int i = 0; i < kDimTiles; ++i)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int d = i * 32 + c * 8 + g * 4;
-        if (d >= dim) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[d + j] = (half_t)(o[i][4 * c + j] * factor);
+        if (d < dim) *(float4_t *)(to + d) = float4_t{o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]} * reference;
       }
+    return;
+  }
+  const float factor = weight == 0.f ? 0.f : reference / weight;
+  half_t *to = a.out + (s.begin + row / a.group) * a.o_token + (int64_t)(h * a.group + row % a.group) * a.o_head;
+#pragma unroll
+  for (int i = 0; i < kDimTiles; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int d = i * 32 + c * 8 + g * 4;
+      if (d >= dim) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[d + j] = (half_t)(o[i][4 * c + j] * factor);
+    }
+}
+
+// A wave adds the parts of a row, a lane 4 dims of it; a workgroup takes 16 rows of a tile.
+__global__ __launch_bounds__(kThreads) void kv_tile_join_kernel(AttentionArgs a) {
+  constexpr int kAhead = 4, kRowsOfJoin = 16;
+  const int dim = a.cache.dim, heads = a.cache.heads, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int b;
+  uint32_t base;
+  KvSequence s;
+  const auto units = [&](const KvSequence &s) { return (uint32_t)(s.count * a.group + kTileRows - 1) / kTileRows * heads; };
+  if (!kv_locate(a.batch, blockIdx.x, units, b, s, base)) return;
+  const int rows = s.count * a.group, tiles = (rows + kTileRows - 1) / kTileRows;
+  const int within = (int)(blockIdx.x - base), h = within % heads, row0 = (tiles - 1 - within / heads) * kTileRows;
+  const int64_t slot0 = (int64_t)blockIdx.x * a.splits;
+  const float *stats = a.parts + (int64_t)a.groups * a.splits * kTileRows * dim;
+  const int d = lane * 4;
+  for (int r = blockIdx.y * kRowsOfJoin + wave; r < min((int)(blockIdx.y + 1) * kRowsOfJoin, rows - row0); r += kThreads / 64) {
+    float most = -__builtin_inff(), weight = 0.f;
+    float4_t value = {};
+    for (int i = 0; i < a.splits; i += kAhead) {
+      float m[kAhead], l[kAhead];
+      float4_t v[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        const int64_t slot = slot0 + min(i + n, a.splits - 1);
+        m[n] = stats[slot * 2 * kTileRows + r], l[n] = stats[slot * 2 * kTileRows + kTileRows + r];
+        v[n] = *(const float4_t *)(a.parts + (slot * kTileRows + r) * dim + min(d, dim - 4));
+      }
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        if (i + n >= a.splits) break;
+        const float next = fmaxf(most, m[n]), zero_point = next == -__builtin_inff() ? 0.f : next;
+        const float keep = __builtin_amdgcn_exp2f(most - zero_point), f = __builtin_amdgcn_exp2f(m[n] - zero_point);
+        value = value * keep + v[n] * f, weight = weight * keep + l[n] * f, most = next;
+      }
+    }
+    if (d < dim) store_row(a, s, h, row0 + r, d, value, weight);
   }
 }
 
@@ -552,20 +611,39 @@ int launch_split(const AttentionArgs &a, hipStream_t stream) {
   return check_launch("kv_split_kernel");
 }
 
+// Workgroups of kv_tile_kernel at most (what the sequences make of the rows only the device knows)
+int64_t tile_groups(const KvBatch &batch, int heads, int group) {
+  return heads * ((int64_t)batch.tokens * group / kTileRows + batch.sequences);
+}
+
+// Workgroups that share a tile: as many as fill the device (one a compute unit above 128 dims, two below), with four blocks at
+// least each, if the longest sequence that the table has room for is there.
+int tile_splits(int64_t groups, int64_t dim, int64_t width) {
+  const int64_t fill = (dim > 128 ? kMostGroups / 2 : kMostGroups) / groups, most = width / 4;
+  const int64_t splits = fill < most ? fill : most;
+  return splits > 1 ? (int)splits : 1;
+}
+
 template <int DP>
-int launch_tile(const AttentionArgs &a, hipStream_t stream) {
+int launch_tile(AttentionArgs &a, hipStream_t stream) {
   const size_t lds = (size_t)2 * 2 * kBlock * DP * sizeof(half_t);
   if (const int rc = allow_lds((const void *)kv_tile_kernel<DP>, lds, "kv_tile_kernel")) return rc;
-  const int64_t groups = a.cache.heads * ((int64_t)a.batch.tokens * a.group / kTileRows + a.batch.sequences);
-  if (groups > 0x7fffffff) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16: too many rows for one launch");
-  kv_tile_kernel<DP><<<(unsigned)groups, kTileThreads, lds, stream>>>(a);
-  return check_launch("kv_tile_kernel");
+  const int64_t groups = tile_groups(a.batch, a.cache.heads, a.group);
+  if (groups > 0x7fffff) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16: too many rows for one launch");
+  a.groups = (int)groups, a.splits = tile_splits(groups, a.cache.dim, a.batch.width);
+  kv_tile_kernel<DP><<<dim3((unsigned)groups, (unsigned)a.splits), kTileThreads, lds, stream>>>(a);
+  const int rc = check_launch("kv_tile_kernel");
+  if (rc != GQ_OK || a.splits == 1) return rc;
+  kv_tile_join_kernel<<<dim3((unsigned)groups, kTileRows / 16), kThreads, 0, stream>>>(a);
+  return check_launch("kv_tile_join_kernel");
 }
 
 }  // namespace
 
+// The larger of what the two kernels keep: 2 x 512 parts of 16 rows, or one of 128 rows for each workgroup of a divided grid
+// (512 at most, 256 above 128 dims).
 int64_t kv_attention_workspace_bytes(int64_t dim) {
-  return (int64_t)2 * kMostGroups * kRows * (dim + 2) * sizeof(float);
+  return (int64_t)(dim > 128 ? kMostGroups / 2 : kMostGroups) * kTileRows * (dim + 2) * sizeof(float);
 }
 
 int launch_kv_attention(const KvCache &cache, const KvBatch &batch, const uint16_t *q, int64_t q_token, int64_t q_head,
@@ -578,8 +656,11 @@ int launch_kv_attention(const KvCache &cache, const KvBatch &batch, const uint16
   a.group = (int)(q_heads / cache.heads);
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.parts = (float *)workspace;
-  a.groups = kMostGroups;
-  // Both kernels are right for every batch; which is faster goes by the rows of a sequence and kv head, on average.
+  a.groups = kMostGroups, a.splits = 1;
+  // Both kernels are right for every batch; which is faster goes by the rows of a sequence and kv head, on average: a tile of 128
+  // costs what kv_split_kernel takes for 16 to 32.  Measured at 32 rows 66 us by kv_split_kernel and 160 us by
+  // kv_tile_kernel (8 sequences of up to 3000, 16 heads of 256), 67 and 94 (32 of up to 3000, 8 heads of 128), at 64
+  // rows 49 and 49 (one of 4000, 16 heads of 256) and 105 and 95 (32 of up to 3000, 8 heads of 128), at 256 rows 90 and 52.
   // (The units of kv_split_kernel have to be countable in 31 bits.)
   const double most_units = (double)cache.heads * ((double)batch.tokens * a.group / kRows + batch.sequences) * (batch.width + 1);
   if (most_units >= 2147483648. || (int64_t)batch.tokens * a.group >= (int64_t)kTileLeast * batch.sequences)

@@ -40,7 +40,7 @@ class KVCacheGQ:
 
     @classmethod
     def from_tensors(cls, k_codes, v_codes, k_scale, v_scale):
-        """A cache on tensors that exist (not copied)."""
+        """A cache on tensors that exist (not copied).  Scales are not negative."""
         import torch
 
         self = cls.__new__(cls)

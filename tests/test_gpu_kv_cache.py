@@ -155,10 +155,10 @@ def test_values_that_are_not_finite_stay_in_their_block(hip, device):
         assert np.isfinite(out[:64]).all() and not np.isfinite(out[64:]).any()
 
 
-def _filled(device, lengths, heads, dim, seed, spare=2):
+def _filled(device, lengths, heads, dim, seed, spare=2, width=0):
     """A cache whose sequences hold drawn codes, everything else the worst that can lie there."""
     rng = np.random.default_rng(seed)
-    table, n_blocks = _table(lengths, seed, spare)
+    table, n_blocks = _table(lengths, seed, spare, width)
     plain = PlainCache(n_blocks, heads, dim)
     for j in range(2):
         plain.codes[j][:] = np.clip(np.rint(rng.normal(0, 40, plain.codes[j].shape)), -127, 127)
@@ -220,6 +220,47 @@ def test_attention_of_sharp_and_flat_scores(hip, device, size, scale):
             _, more = attend(q[rows], -k, v, n - (offsets[b + 1] - offsets[b]), -scale)
             room = np.maximum(room, more)
         assert_within(got[rows], want, room, f"sequence {b}")
+
+
+@pytest.mark.parametrize("scale", [None, 0.0, -0.4, 3.0])
+@pytest.mark.parametrize("lengths,fresh,heads,group,dim,width", [([600], [90], 1, 1, 64, 64), ([400, 90], [120, 90], 2, 2, 128, 40),
+                                                                  ([257], [257], 1, 1, 256, 100), ([700], [33], 1, 4, 80, 12)])
+def test_attention_of_many_rows(hip, device, lengths, fresh, heads, group, dim, width, scale):
+    """Prompts whose few tiles are divided over the keys (a wide table), at scales that turn, flatten and sharpen the scores;
+    value scales of neighbouring blocks that differ by a thousand, and blocks of zeros."""
+    cache, plain, table = _filled(device, lengths, heads, dim, 7 * dim + len(lengths), width=width)
+    for j, c in enumerate((cache.k_scale, cache.v_scale)):
+        for b, n in enumerate(lengths):
+            for p in range(n // BLOCK):
+                plain.scale[j][table[b, p]] *= [1, 1e-3, 0, 3, 1e3][(p + j) % 5] if j else [1, 0, 2][p % 3]
+        c.copy_(torch.from_numpy(plain.scale[j]).to(device))
+    offsets = np.concatenate([[0], np.cumsum(fresh)])
+    q = _normal(dim, offsets[-1], heads * group, dim)
+    got = kv_cache_attention(torch.from_numpy(q).to(device), cache, *_int32(device, offsets, lengths, table), scale=scale).cpu().numpy()
+    for b, n in enumerate(lengths):
+        rows = slice(offsets[b], offsets[b + 1])
+        k, v = plain.values(0, b, n, table), plain.values(1, b, n, table)
+        want, room = attend(q[rows], k, v, n - fresh[b], dim ** -0.5 if scale is None else scale)
+        if scale is not None and scale < 0:
+            _, more = attend(q[rows], -k, v, n - fresh[b], -scale)
+            room = np.maximum(room, more)
+        assert_within(got[rows], want, room, f"sequence {b}")
+
+
+def test_many_rows_beside_a_block_that_is_not_finite(hip, device):
+    """Rows in front of a block whose scales are not finite are as if it were not there."""
+    for bad in (np.inf, np.nan):
+        lengths, dim = [200], 64
+        cache, plain, table = _filled(device, lengths, 1, dim, 41)
+        q = torch.from_numpy(_normal(2, 200, 1, dim)).to(device)
+        batch = _int32(device, [0, 200], lengths, table)
+        want = kv_cache_attention(q, cache, *batch).cpu().numpy()
+        for scale in (cache.k_scale, cache.v_scale):
+            before = scale.clone()
+            scale[table[0, 2]] = bad
+            got = kv_cache_attention(q, cache, *batch).cpu().numpy()
+            assert np.array_equal(got[:128], want[:128]) and not np.isfinite(got[128:]).any(1).any()
+            scale.copy_(before)
 
 
 def test_attention_strides_streams_and_repeats(hip, device):
