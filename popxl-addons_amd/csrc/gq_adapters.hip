@@ -184,6 +184,54 @@ __device__ __forceinline__ half8_t load8_any(const half_t *row, int64_t at, int6
   return load8<false>(row + at, size - at);
 }
 
+// The gradients contract the other axis of each weight: both are turned first, [rows][columns] to [columns][rows] for every
+// adapter that has rows (a gradient of 4 bytes an element is written for every one of them, so this never dominates), by workgroups
+// of the launch that forms x A^T, which does not need them: a launch less, and its time is hidden.
+struct TurnArgs {
+  const half_t *from[2];
+  half_t *to[2];
+  int64_t rows[2], columns[2];
+  const int *parts_of;
+  int pieces, adapters;  // of the grid
+  bool wide;  // rows and columns of both are multiples of 8, 16-byte aligned
+};
+
+// workgroup `group` of a.pieces x adapters x 2; 64 x 72 of LDS
+__device__ __forceinline__ void turn_weights(const TurnArgs &a, int group, half_t (*piece)[72]) {
+  const int first = group % a.pieces, adapter = group / a.pieces % a.adapters, which = group / a.pieces / a.adapters, tid = threadIdx.x;
+  if (a.parts_of[2 * adapter + 1] == 0) return;
+  const int64_t rows = which ? a.rows[1] : a.rows[0], columns = which ? a.columns[1] : a.columns[0];
+  const int64_t across = (columns + 63) / 64, pieces = (rows + 63) / 64 * across;
+  const half_t *from = (which ? a.from[1] : a.from[0]) + adapter * rows * columns;
+  half_t *to = (which ? a.to[1] : a.to[0]) + adapter * rows * columns;
+  for (int64_t n = first; n < pieces; n += a.pieces) {
+    const int64_t r0 = n / across * 64, c0 = n % across * 64;
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < 64 * 8; i += kThreads) {
+      const int64_t r = r0 + i / 8, c = c0 + i % 8 * 8;
+      if (r >= rows) continue;
+      *(half8_t *)&piece[i / 8][i % 8 * 8] = a.wide ? load8<true>(from + r * columns + c, columns - c) : load8<false>(from + r * columns + c, columns - c);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = tid; i < 64 * 8; i += kThreads) {
+      const int64_t c = c0 + i / 8, r = r0 + i % 8 * 8;
+      if (c >= columns) continue;
+      half8_t v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = piece[i % 8 * 8 + j][i / 8];
+      if (a.wide) {
+        if (r < rows) *(half8_t *)(to + c * rows + r) = v;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (r + j < rows) to[c * rows + r + j] = v[j];
+      }
+    }
+  }
+}
+
 struct DownArgs {
   const half_t *x, *w;  // w: [adapters][rank][features]
   int64_t x_stride;
@@ -192,7 +240,8 @@ struct DownArgs {
   float *v;     // [splits][rows][kRank]
   float *most;  // [splits][tiles]: largest magnitudes (NULL: nobody asks)
   int64_t rows, features, split;  // features of one split, a multiple of 128
-  int rank, most_tiles;
+  int rank, most_tiles, splits;
+  TurnArgs turn;  // what the workgroups behind most_tiles x splits do
 };
 
 // kRank: rank rounded up to 32, 64 or 128; kTiles x 16 rows.  The four waves of a workgroup have a quarter of its features
@@ -203,10 +252,15 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   constexpr int kRankTiles = kRank / 16;
   extern __shared__ float shared[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-  if ((int)blockIdx.x >= *a.tile_count) return;
-  const AdapterTile tile = a.tiles[blockIdx.x];
+  const int split = blockIdx.x / a.most_tiles, index = blockIdx.x - split * a.most_tiles;
+  if (split >= a.splits) {
+    turn_weights(a.turn, blockIdx.x - a.splits * a.most_tiles, (half_t(*)[72])shared);
+    return;
+  }
+  if (index >= *a.tile_count) return;
+  const AdapterTile tile = a.tiles[index];
   if (tile.adapter < 0) return;
-  const int64_t mine = a.split / kWaves, from = min(a.features, blockIdx.y * a.split + wave * mine), to = min(a.features, from + mine);
+  const int64_t mine = a.split / kWaves, from = min(a.features, split * a.split + wave * mine), to = min(a.features, from + mine);
   const half_t *w = a.w + (int64_t)tile.adapter * a.rank * a.features;
   const half_t *x[kTiles], *wr[kRankTiles];
 #pragma unroll
@@ -234,14 +288,15 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
       for (int u = 0; u < 2; ++u) wf[set][r][u] = load8_any<kWide>(wr[r], k + 32 * u, a.features);
   };
   const auto multiply = [&](int set, int64_t k) {
-    if (k + 64 > to) {  // values behind the range are zeros
+    if (k + 64 > to) {  // values behind the range are zeros on both sides (`to` is a multiple of 8 or the row's end)
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
+      for (int u = 0; u < 2; ++u) {
+        if (k + 32 * u + g * 8 < to) continue;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int t = 0; t < kTiles; ++t) xf[set][t][u] = half8_t{};
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (k + 32 * u + g * 8 + j >= to) xf[set][t][u][j] = (half_t)0.f;
+        for (int r = 0; r < kRankTiles; ++r) wf[set][r][u] = half8_t{};
+      }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -255,7 +310,7 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   };
   // Tiles start at different places of their range: rows are often a power of two apart, and tiles that walked their columns in
   // step would keep asking the same few memory channels (8192 rows of 16384: 87 us, 74 us so).
-  const int steps = (int)((to - from + 63) / 64), turn = steps > 0 ? blockIdx.x * 5 % steps : 0;
+  const int steps = (int)((to - from + 63) / 64), turn = steps > 0 ? index * 5 % steps : 0;
   const auto place = [&](int i) {
     const int at = turn + min(i, steps - 1);
     return from + 64 * (int64_t)(at < steps ? at : at - steps);
@@ -270,7 +325,7 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
     }
   }
   // sum of the four waves, 16 rows at a time: [waves][16 rows][kRank + 4]
-  float *v = a.v + ((int64_t)blockIdx.y * a.rows + tile.begin) * kRank;
+  float *v = a.v + ((int64_t)split * a.rows + tile.begin) * kRank;
   float most = 0.f;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
@@ -299,24 +354,9 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
     if (lane == 0) shared[wave] = most;
     __syncthreads();
     if (threadIdx.x == 0)
-      a.most[(int64_t)blockIdx.y * a.most_tiles + blockIdx.x] = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
+      a.most[(int64_t)split * a.most_tiles + index] = fmaxf(fmaxf(shared[0], shared[1]), fmaxf(shared[2], shared[3]));
   }
 }
-
-struct UpArgs {
-  const float *v;   // [splits][rows][kRank]
-  const half_t *w;  // [adapters][features][rank]
-  const float *scaling;
-  const half_t *y;  // out where there is none
-  half_t *out;
-  int64_t y_stride, out_stride;
-  bool has_y;
-  const AdapterTile *tiles;
-  const int *tile_count, *order;
-  int64_t rows, features, range;  // features of one workgroup, a multiple of 256
-  int rank, splits, act;
-  bool skip_rows_without;  // out is y and there is no activation: rows without an adapter are done
-};
 
 // two binary16 numbers whose sum is v to 22 bits of 1
 __device__ __forceinline__ void split_of(float v, half_t &hi, half_t &lo) {
@@ -363,6 +403,94 @@ __device__ __forceinline__ float4_t sum_of_splits(const float *p, int64_t stride
   return sum;
 }
 
+struct OuterSide {
+  const half_t *x;  // [rows][features]
+  int64_t x_stride, features;
+  const float *v;     // [splits][rows][kRank]
+  const float *most;  // [splits][tiles]
+  int splits;
+  half_t *operand;  // [row of operand_row / 32][hi, lo][16 ranks][lane][8]: 1 KiB for a wave's load
+  float *back;      // [segments]
+  float *grad;      // [adapters][rank][features], turned: [adapters][features][rank]
+  float *parts;     // [parts], the same
+  bool turned;
+};
+
+struct OuterArgs {
+  OuterSide side[2];
+  const AdapterTile *segments;
+  const int *segment_count, *order, *parts_of;
+  const float *scaling;
+  int64_t rows;
+  int rank, adapters, most_tiles, most_segments;
+  bool large;
+};
+
+// Where a segment's rows begin in the operands: pieces of 64 rows, the segments apart (their rows are consecutive in the order,
+// and 64 rows more for each keep rounded ones from meeting).
+__device__ __forceinline__ int64_t operand_row(int segment, int begin) { return (int64_t)(begin / 64 + segment) * 64; }
+
+// v of a segment as the other product's operand: 64 rows a workgroup, summed over the splits, scaled by the segment's power of
+// two, split, transposed.  The power comes from the largest part times the number of splits, which is no less than the
+// largest sum; what it is too large by costs that many of the 22 bits.
+// Workgroup `group` of segments x pieces x 2; [2][kRank][72] of LDS.
+template <int kRank>
+__device__ __forceinline__ void make_operand(const OuterArgs &a, int group, half_t *shared) {
+  constexpr int kRow = 64 + 8;
+  half_t(*piece)[kRank][kRow] = (half_t(*)[kRank][kRow])shared;
+  const int segment = group % a.most_segments, part = group / a.most_segments;
+  const OuterSide &side = part & 1 ? a.side[1] : a.side[0];
+  if (segment >= *a.segment_count) return;
+  const AdapterTile seg = a.segments[segment];
+  const int i0 = (part >> 1) * 64, tid = threadIdx.x, lane = tid & 63;
+  if (i0 >= seg.count) return;
+  const int per_tile = a.large ? kAdapterLargeTile : kAdapterSmallTile, tiles = (seg.count + per_tile - 1) / per_tile;
+  const float *most_of = side.most + (a.large ? seg.first_large : seg.first);
+  float most = 0.f;
+  for (int n = lane; n < tiles * side.splits; n += 64) most = fmaxf(most, most_of[(int64_t)(n / tiles) * a.most_tiles + n % tiles]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  most *= side.splits;
+  float back;
+  const float power = normal_power(most, back);
+  if (i0 == 0 && tid == 0) side.back[segment] = back * a.scaling[seg.adapter];
+  for (int n = tid; n < 64 * kRank / 4; n += kThreads) {
+    const int i = n / (kRank / 4), r = n % (kRank / 4) * 4;
+    float4_t sum = {};
+    if (i0 + i < seg.count) sum = sum_of_splits(side.v + (int64_t)(seg.begin + i0 + i) * kRank + r, a.rows * kRank, side.splits);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      half_t h, l;
+      split_of(sum[j] * power, h, l);
+      piece[0][r + j][i] = h, piece[1][r + j][i] = l;
+    }
+  }
+  __syncthreads();
+  half_t *to = side.operand + (operand_row(segment, seg.begin) + i0) * 2 * kRank;
+  for (int n = tid; n < 2 * 2 * kRank * 4; n += kThreads) {
+    const int m = n % 16, g = n / 16 % 4, r = n / 64 % (kRank / 16), which = n / (kRank * 4) % 2, step = n / (kRank * 8);
+    *(half8_t *)(to + n * 8) = *(const half8_t *)&piece[which][r * 16 + m][step * 32 + g * 8];
+  }
+}
+
+struct UpArgs {
+  const float *v;   // [splits][rows][kRank]
+  const half_t *w;  // [adapters][features][rank]
+  const float *scaling;
+  const half_t *y;  // out where there is none
+  half_t *out;
+  int64_t y_stride, out_stride;
+  bool has_y;
+  const AdapterTile *tiles;
+  const int *tile_count, *order;
+  int64_t rows, features, range;  // features of one workgroup, a multiple of 256
+  int rank, splits, act;
+  int ranges;
+  OuterArgs outer;  // gradients: the workgroups behind tiles x ranges make its operand
+  int most_tiles;
+  bool skip_rows_without;  // out is y and there is no activation: rows without an adapter are done
+};
+
 // The workgroup sums its rows' v over the splits into LDS, where its waves take their operands from.  Then wave w takes 64
 // features at a time: row 4 g' + i of operand tile f is feature 32 (f / 2) + 8 g' + 4 (f % 2) + i, so that a lane ends with 8
 // consecutive features of one row in each half (16-byte loads and stores, 64 bytes of a row together).  The weights and y of the next
@@ -370,17 +498,22 @@ __device__ __forceinline__ float4_t sum_of_splits(const float *p, int64_t stride
 template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
   constexpr int kChunks = kRank / 32, kRow = kRank + 4;
-  __shared__ float v[kTiles * 16 * kRow];
+  extern __shared__ float v[];  // [kTiles x 16 rows][kRow]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
-  if ((int)blockIdx.x >= *a.tile_count) return;
-  const AdapterTile tile = a.tiles[blockIdx.x];
+  const int range = blockIdx.x / a.most_tiles, index = blockIdx.x - range * a.most_tiles;
+  if (range >= a.ranges) {
+    make_operand<kRank>(a.outer, blockIdx.x - a.ranges * a.most_tiles, (half_t *)v);
+    return;
+  }
+  if (index >= *a.tile_count) return;
+  const AdapterTile tile = a.tiles[index];
   const bool with = tile.adapter >= 0;
   if (!with && a.skip_rows_without) return;
   const half_t *w = a.w + (int64_t)max(tile.adapter, 0) * a.rank * a.features;
   const float scaling = with ? a.scaling[tile.adapter] : 0.f;
-  const int64_t from = blockIdx.y * a.range, to = min(a.features, from + a.range), first = from + wave * 64;
+  const int64_t from = range * a.range, to = min(a.features, from + a.range), first = from + wave * 64;
   // (tiles start at different pieces of the range and loads have no conditions, as in adapter_down_kernel)
-  const int pieces = first < to ? (int)((to - first + kWaves * 64 - 1) / (kWaves * 64)) : 0, turn = pieces > 0 ? blockIdx.x * 5 % pieces : 0;
+  const int pieces = first < to ? (int)((to - first + kWaves * 64 - 1) / (kWaves * 64)) : 0, turn = pieces > 0 ? index * 5 % pieces : 0;
   const auto place = [&](int i) {
     if (pieces == 0) return (int64_t)0;  // (a wave without features still loads, and drops, the first ones)
     const int at = turn + min(i, pieces - 1);
@@ -494,116 +627,6 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   }
 }
 
-// The gradients contract the other axis of each weight: both are turned first, [rows][columns] to [columns][rows] for every
-// adapter that has rows (a gradient of 4 bytes an element is written for every one of them, so this never dominates).
-struct TurnArgs {
-  const half_t *from[2];
-  half_t *to[2];
-  int64_t rows[2], columns[2];
-  const int *parts_of;
-  bool wide;  // rows and columns of both are multiples of 8, 16-byte aligned
-};
-
-__global__ __launch_bounds__(kThreads) void adapter_turn_kernel(TurnArgs a) {
-  __shared__ half_t piece[64][72];
-  const int which = blockIdx.z, adapter = blockIdx.y, tid = threadIdx.x;
-  if (a.parts_of[2 * adapter + 1] == 0) return;
-  const int64_t rows = which ? a.rows[1] : a.rows[0], columns = which ? a.columns[1] : a.columns[0];
-  const int64_t across = (columns + 63) / 64, pieces = (rows + 63) / 64 * across;
-  const half_t *from = (which ? a.from[1] : a.from[0]) + adapter * rows * columns;
-  half_t *to = (which ? a.to[1] : a.to[0]) + adapter * rows * columns;
-  for (int64_t n = blockIdx.x; n < pieces; n += gridDim.x) {
-    const int64_t r0 = n / across * 64, c0 = n % across * 64;
-    __syncthreads();
-#pragma unroll
-    for (int i = tid; i < 64 * 8; i += kThreads) {
-      const int64_t r = r0 + i / 8, c = c0 + i % 8 * 8;
-      if (r >= rows) continue;
-      *(half8_t *)&piece[i / 8][i % 8 * 8] = a.wide ? load8<true>(from + r * columns + c, columns - c) : load8<false>(from + r * columns + c, columns - c);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = tid; i < 64 * 8; i += kThreads) {
-      const int64_t c = c0 + i / 8, r = r0 + i % 8 * 8;
-      if (c >= columns) continue;
-      half8_t v;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = piece[i % 8 * 8 + j][i / 8];
-      if (a.wide) {
-        if (r < rows) *(half8_t *)(to + c * rows + r) = v;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (r + j < rows) to[c * rows + r + j] = v[j];
-      }
-    }
-  }
-}
-
-struct OuterSide {
-  const half_t *x;  // [rows][features]
-  int64_t x_stride, features;
-  const float *v;     // [splits][rows][kRank]
-  const float *most;  // [splits][tiles]
-  int splits;
-  half_t *operand;  // [segments][steps of 32 rows][hi, lo][16 ranks][lane][8]: 1 KiB for a wave's load
-  float *back;      // [segments]
-  float *grad;      // [adapters][rank][features], turned: [adapters][features][rank]
-  float *parts;     // [parts], the same
-  bool turned;
-};
-
-struct OuterArgs {
-  OuterSide side[2];
-  const AdapterTile *segments;
-  const int *segment_count, *order, *parts_of;
-  const float *scaling;
-  int64_t rows;
-  int rank, adapters, most_tiles;
-  bool large;
-};
-
-// v of a segment as the other product's operand: 64 rows a workgroup, summed over the splits, scaled by the segment's power of
-// two, split, transposed.  The power comes from the largest part times the number of splits, which is no less than the
-// largest sum; what it is too large by costs that many of the 22 bits.
-template <int kRank>
-__global__ __launch_bounds__(kThreads) void adapter_operand_kernel(OuterArgs a) {
-  constexpr int kRow = 64 + 8;
-  __shared__ half_t piece[2][kRank][kRow];
-  const OuterSide &side = blockIdx.z ? a.side[1] : a.side[0];
-  if ((int)blockIdx.x >= *a.segment_count) return;
-  const AdapterTile seg = a.segments[blockIdx.x];
-  const int i0 = blockIdx.y * 64, tid = threadIdx.x, lane = tid & 63;
-  if (i0 >= seg.count) return;
-  const int per_tile = a.large ? kAdapterLargeTile : kAdapterSmallTile, tiles = (seg.count + per_tile - 1) / per_tile;
-  const float *most_of = side.most + (a.large ? seg.first_large : seg.first);
-  float most = 0.f;
-  for (int n = lane; n < tiles * side.splits; n += 64) most = fmaxf(most, most_of[(int64_t)(n / tiles) * a.most_tiles + n % tiles]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  most *= side.splits;
-  float back;
-  const float power = normal_power(most, back);
-  if (i0 == 0 && tid == 0) side.back[blockIdx.x] = back * a.scaling[seg.adapter];
-  for (int n = tid; n < 64 * kRank / 4; n += kThreads) {
-    const int i = n / (kRank / 4), r = n % (kRank / 4) * 4;
-    float4_t sum = {};
-    if (i0 + i < seg.count) sum = sum_of_splits(side.v + (int64_t)(seg.begin + i0 + i) * kRank + r, a.rows * kRank, side.splits);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      half_t h, l;
-      split_of(sum[j] * power, h, l);
-      piece[0][r + j][i] = h, piece[1][r + j][i] = l;
-    }
-  }
-  __syncthreads();
-  half_t *to = side.operand + ((int64_t)blockIdx.x * kAdapterSegment + i0) * 2 * kRank;
-  for (int n = tid; n < 2 * 2 * kRank * 4; n += kThreads) {
-    const int m = n % 16, g = n / 16 % 4, r = n / 64 % (kRank / 16), which = n / (kRank * 4) % 2, step = n / (kRank * 8);
-    *(half8_t *)(to + n * 8) = *(const half8_t *)&piece[which][r * 16 + m][step * 32 + g * 8];
-  }
-}
-
 // 128 features of one segment's product; the four waves take every fourth 32 rows and meet in LDS.  The rows are loaded as
 // they lie (8 features a lane, 8 rows) and paired in registers: operand c has feature 8 m + c, so that a lane ends with 8
 // consecutive features of 4 ranks.  Rows are loaded two steps ahead, the operand one: one wave a SIMD with 512 registers keeps
@@ -624,7 +647,8 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
   for (int n = threadIdx.x; n < seg.count; n += kThreads) order[n] = a.order[seg.begin + n];
   __syncthreads();
   // (in the order of the loads: rows of it a power of two apart would all be asked of one memory channel)
-  const half_t *operand = side.operand + (int64_t)blockIdx.x * kAdapterSegment * 2 * kRank + rank0 * 32 + lane * 8;
+  const half_t *operand = side.operand + operand_row(blockIdx.x, seg.begin) * 2 * kRank + rank0 * 32 + lane * 8;
+  const int last_step = (seg.count - 1) / 32 * 32;
   const int64_t f = (int64_t)blockIdx.y * 128 + m * 8;
 
   float4_t acc[kRankTiles][8];
@@ -644,7 +668,7 @@ __global__ __launch_bounds__(kThreads, 1) void adapter_outer_kernel(OuterArgs a)
     }
   };
   const auto load_operand = [&](int set, int i0) {
-    const half_t *at = operand + (int64_t)min(i0, kAdapterSegment - 32) * 2 * kRank;
+    const half_t *at = operand + (int64_t)min(i0, last_step) * 2 * kRank;
 #pragma unroll
     for (int r = 0; r < kRankTiles; ++r) {
       h[set][r] = *(const half8_t *)(at + r * 512);
@@ -753,15 +777,18 @@ int allow_lds(const void *kernel, size_t bytes, const char *who) {
 }
 
 template <int kRank, int kTiles, bool kWide>
-int start_down(const DownArgs &a, int64_t tiles, int64_t splits, hipStream_t stream) {
-  const size_t lds = (size_t)kWaves * 16 * (kRank + 4) * sizeof(float);
-  adapter_down_kernel<kRank, kTiles, kWide><<<dim3((unsigned)tiles, (unsigned)splits), kThreads, lds, stream>>>(a);
+int start_down(const DownArgs &a, int64_t turns, hipStream_t stream) {
+  const size_t sums = (size_t)kWaves * 16 * (kRank + 4) * sizeof(float), turned = turns ? 64 * 72 * sizeof(half_t) : 0;
+  adapter_down_kernel<kRank, kTiles, kWide>
+      <<<(unsigned)((int64_t)a.most_tiles * a.splits + turns), kThreads, sums > turned ? sums : turned, stream>>>(a);
   return check_launch("adapter_down_kernel");
 }
 
 template <int kRank, int kTiles, bool kWide>
-int start_up(const UpArgs &a, int64_t tiles, int64_t ranges, hipStream_t stream) {
-  adapter_up_kernel<kRank, kTiles, kWide><<<dim3((unsigned)tiles, (unsigned)ranges), kThreads, 0, stream>>>(a);
+int start_up(const UpArgs &a, int64_t operands, hipStream_t stream) {
+  const size_t rows = (size_t)kTiles * 16 * (kRank + 4) * sizeof(float), operand = operands ? (size_t)2 * kRank * 72 * sizeof(half_t) : 0;
+  adapter_up_kernel<kRank, kTiles, kWide>
+      <<<(unsigned)((int64_t)a.most_tiles * a.ranges + operands), kThreads, rows > operand ? rows : operand, stream>>>(a);
   return check_launch("adapter_up_kernel");
 }
 
@@ -776,19 +803,21 @@ int start_up(const UpArgs &a, int64_t tiles, int64_t ranges, hipStream_t stream)
 bool aligned16(const void *p) { return (uintptr_t)p % 16 == 0; }
 
 int launch_down(const Batch &b, const half_t *x, int64_t x_stride, const half_t *w, int64_t features, int64_t rank, float *v, float *most,
-                int64_t splits, hipStream_t stream) {
-  DownArgs a;
+                int64_t splits, const TurnArgs *turn, hipStream_t stream) {
+  DownArgs a = {};
   a.x = x, a.w = w, a.x_stride = x_stride, a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0);
   a.order = b.words + b.plan.order, a.v = v, a.most = most, a.rows = b.plan.rows, a.features = features, a.rank = (int)rank;
-  a.split = round_up((features + splits - 1) / splits, 128), a.most_tiles = (int)b.most_tiles();
+  a.split = round_up((features + splits - 1) / splits, 128), a.most_tiles = (int)b.most_tiles(), a.splits = (int)splits;
+  if (turn) a.turn = *turn;
+  const int64_t turns = turn ? (int64_t)turn->pieces * turn->adapters * 2 : 0;
   const bool large = b.large, wide = aligned16(x) && aligned16(w) && x_stride % 8 == 0 && features % 8 == 0;
   const int kRankClass = rank_class(rank);
-  return GQ_BY_SHAPE(start_down, a, b.most_tiles(), splits, stream);
+  return GQ_BY_SHAPE(start_down, a, turns, stream);
 }
 
 int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, const float *scaling, const half_t *y, int64_t y_stride,
-              half_t *out, int64_t out_stride, int64_t features, int64_t rank, int act, hipStream_t stream) {
-  UpArgs a;
+              half_t *out, int64_t out_stride, int64_t features, int64_t rank, int act, const OuterArgs *outer, hipStream_t stream) {
+  UpArgs a = {};
   a.v = v, a.w = w, a.scaling = scaling, a.has_y = y != nullptr, a.out = out, a.out_stride = out_stride;
   a.y = y ? y : out, a.y_stride = y ? y_stride : out_stride;
   a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0), a.order = b.words + b.plan.order;
@@ -796,26 +825,25 @@ int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, c
   a.skip_rows_without = y == out && y_stride == out_stride && act == GQ_ACT_NONE;
   const int64_t tiles = b.most_tiles(), most = (features + 255) / 256, want = (1024 + tiles - 1) / tiles;
   a.range = round_up((features + (want < most ? want : most) - 1) / (want < most ? want : most), 256);
-  const int64_t ranges = (features + a.range - 1) / a.range;
+  a.most_tiles = (int)tiles, a.ranges = (int)((features + a.range - 1) / a.range);
+  if (outer) a.outer = *outer;
+  const int64_t longest = b.plan.rows < kAdapterSegment ? b.plan.rows : kAdapterSegment;
+  const int64_t operands = outer ? outer->most_segments * ((longest + 63) / 64) * 2 : 0;
   const bool large = b.large, wide = aligned16(y) && aligned16(out) && aligned16(w) && y_stride % 8 == 0 && out_stride % 8 == 0 &&
                                      features % 8 == 0 && rank % 8 == 0;
   const int kRankClass = rank_class(rank);
-  return GQ_BY_SHAPE(start_up, a, tiles, ranges, stream);
+  return GQ_BY_SHAPE(start_up, a, operands, stream);
 }
 
 template <int kRank>
 int launch_outer(const OuterArgs &a, const PlanLayout &plan, bool wide, hipStream_t stream) {
   const int64_t features = a.side[0].features > a.side[1].features ? a.side[0].features : a.side[1].features;
-  const int64_t longest = plan.rows < kAdapterSegment ? plan.rows : kAdapterSegment;
-  adapter_operand_kernel<kRank><<<dim3((unsigned)plan.most_segments, (unsigned)((longest + 63) / 64), 2), kThreads, 0, stream>>>(a);
-  int rc = check_launch("adapter_operand_kernel");
-  if (rc != GQ_OK) return rc;
   const dim3 grid((unsigned)plan.most_segments, (unsigned)((features + 127) / 128), 2 * (kRank > 64 ? 2 : 1));
   if (wide)
     adapter_outer_kernel<kRank, true><<<grid, kThreads, 0, stream>>>(a);
   else
     adapter_outer_kernel<kRank, false><<<grid, kThreads, 0, stream>>>(a);
-  rc = check_launch("adapter_outer_kernel");
+  const int rc = check_launch("adapter_outer_kernel");
   if (rc != GQ_OK) return rc;
   const int64_t each = (a.rank * features + kThreads - 1) / kThreads;
   adapter_sum_kernel<<<dim3((unsigned)(each < 1024 ? each : 1024), (unsigned)a.adapters, 2), kThreads, 0, stream>>>(a);
@@ -836,7 +864,7 @@ struct GradLayout {
     for (int i = 0; i < 2; ++i) {
       most[i] = take((i ? out_splits : in_splits) * most_tiles * 4);
       turned[i] = take(plan.adapters * rank * (i ? out : in) * 2);
-      operand[i] = take(plan.most_segments * 2 * width * kAdapterSegment * 2), back[i] = take(plan.most_segments * 4);
+      operand[i] = take((plan.rows + 64 * (plan.most_segments + 1)) * 2 * width * 2), back[i] = take(plan.most_segments * 4);
       parts[i] = take(plan.most_parts * rank * (i ? out : in) * 4);
     }
     bytes = at;
@@ -867,10 +895,10 @@ int launch_adapter_apply(const gq_adapters &w, const void *plan, int64_t rows, c
                          int64_t y_stride, uint16_t *out, int64_t out_stride, int act, void *workspace, hipStream_t stream) {
   const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows)};
   const int64_t splits = down_splits(b.most_tiles(), w.in_features);
-  const int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, w.in_features, w.rank, (float *)workspace, nullptr, splits, stream);
+  const int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, w.in_features, w.rank, (float *)workspace, nullptr, splits, nullptr, stream);
   if (rc != GQ_OK) return rc;
   return launch_up(b, (const float *)workspace, splits, (const half_t *)w.up, w.scaling, (const half_t *)y, y_stride, (half_t *)out, out_stride,
-                   w.out_features, w.rank, act, stream);
+                   w.out_features, w.rank, act, nullptr, stream);
 }
 
 int64_t adapter_grad_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t out, int64_t rank) {
@@ -888,18 +916,15 @@ int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, co
   const GradLayout l(b.plan, tiles, in, out, w.rank, in_splits, out_splits);
   char *ws = (char *)workspace;
   half_t *down_turned = (half_t *)(ws + l.turned[0]), *up_turned = (half_t *)(ws + l.turned[1]);
-  const TurnArgs turn = {{(const half_t *)w.down, (const half_t *)w.up}, {down_turned, up_turned}, {w.rank, out}, {in, w.rank},
-                         b.words + b.plan.parts, (w.rank | in | out) % 8 == 0 && aligned16(w.down) && aligned16(w.up)};
   const int64_t pieces = ((in > out ? in : out) + 63) / 64 * ((w.rank + 63) / 64);
-  adapter_turn_kernel<<<dim3((unsigned)(pieces < 512 ? pieces : 512), (unsigned)w.n_adapters, 2), kThreads, 0, stream>>>(turn);
-  int rc = check_launch("adapter_turn_kernel");
+  const TurnArgs turn = {{(const half_t *)w.down, (const half_t *)w.up}, {down_turned, up_turned}, {w.rank, out}, {in, w.rank},
+                         b.words + b.plan.parts, (int)(pieces < 512 ? pieces : 512), (int)w.n_adapters,
+                         (w.rank | in | out) % 8 == 0 && aligned16(w.down) && aligned16(w.up)};
+  int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, in, w.rank, (float *)(ws + l.v), (float *)(ws + l.most[0]), in_splits,
+                       &turn, stream);
   if (rc == GQ_OK)
-    rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, in, w.rank, (float *)(ws + l.v), (float *)(ws + l.most[0]), in_splits, stream);
-  if (rc == GQ_OK)
-    rc = launch_down(b, (const half_t *)dy, dy_stride, up_turned, out, w.rank, (float *)(ws + l.dv), (float *)(ws + l.most[1]), out_splits, stream);
-  if (rc == GQ_OK)
-    rc = launch_up(b, (const float *)(ws + l.dv), out_splits, down_turned, w.scaling, (const half_t *)dx, dx_stride, (half_t *)dx_out, dx_out_stride,
-                   in, w.rank, GQ_ACT_NONE, stream);
+    rc = launch_down(b, (const half_t *)dy, dy_stride, up_turned, out, w.rank, (float *)(ws + l.dv), (float *)(ws + l.most[1]), out_splits, nullptr,
+                     stream);
   if (rc != GQ_OK) return rc;
   OuterArgs a;
   // dA: the rows of x with dv;  dB: the rows of dy with v
@@ -913,7 +938,10 @@ int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, co
   }
   a.segments = (const AdapterTile *)(b.words + b.plan.segments), a.segment_count = b.words + b.plan.counts + 2;
   a.order = b.words + b.plan.order, a.parts_of = b.words + b.plan.parts, a.scaling = w.scaling;
-  a.rows = rows, a.rank = (int)w.rank, a.adapters = (int)w.n_adapters, a.most_tiles = (int)tiles, a.large = b.large;
+  a.rows = rows, a.rank = (int)w.rank, a.adapters = (int)w.n_adapters, a.most_tiles = (int)tiles, a.most_segments = (int)b.plan.most_segments, a.large = b.large;
+  rc = launch_up(b, (const float *)(ws + l.dv), out_splits, down_turned, w.scaling, (const half_t *)dx, dx_stride, (half_t *)dx_out, dx_out_stride,
+                 in, w.rank, GQ_ACT_NONE, &a, stream);
+  if (rc != GQ_OK) return rc;
   const bool wide = aligned16(x) && aligned16(dy) && (x_stride | dy_stride | in | out) % 8 == 0;
   return rank_class(w.rank) == 32   ? launch_outer<32>(a, b.plan, wide, stream)
          : rank_class(w.rank) == 64 ? launch_outer<64>(a, b.plan, wide, stream)

@@ -263,6 +263,20 @@ def test_many_rows_beside_a_block_that_is_not_finite(hip, device):
             scale.copy_(before)
 
 
+@pytest.mark.parametrize("fresh", [3, 100])
+def test_queries_that_are_not_finite_stay_in_their_row(hip, device, fresh):
+    lengths, dim = [150], 64
+    cache, plain, table = _filled(device, lengths, 1, dim, 51)
+    q = _normal(3, fresh, 2, dim)
+    batch = _int32(device, [0, fresh], lengths, table)
+    want = kv_cache_attention(torch.from_numpy(q).to(device), cache, *batch).cpu().numpy()
+    q[0, 1, 5], q[2, 0, 63], q[1, 1, 0] = np.nan, np.inf, -np.inf
+    got = kv_cache_attention(torch.from_numpy(q).to(device), cache, *batch).cpu().numpy()
+    bad = np.zeros((fresh, 2), bool)
+    bad[0, 1] = bad[2, 0] = bad[1, 1] = True
+    assert np.array_equal(got[~bad], want[~bad]) and np.isnan(got[bad]).any(1).all()
+
+
 def test_attention_strides_streams_and_repeats(hip, device):
     lengths, fresh, heads, group, dim = [700, 65, 130], [1, 3, 20], 2, 4, 64
     cache, plain, table = _filled(device, lengths, heads, dim, 21)
