@@ -497,8 +497,8 @@ struct UpArgs {
 // piece are loaded before and among this one's products.
 template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
-  constexpr int kChunks = kRank / 32, kRow = kRank + 4;
-  extern __shared__ float v[];  // [kTiles x 16 rows][kRow]
+  constexpr int kChunks = kRank / 32, kRow = kRank + 4, kTurned = 64 + 4;
+  extern __shared__ float v[];  // [kTiles x 16 rows][kRow], then [waves][16 rows][kTurned]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15, g = lane >> 4;
   const int range = blockIdx.x / a.most_tiles, index = blockIdx.x - range * a.most_tiles;
   if (range >= a.ranges) {
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   };
 
   half8_t wf[2][4][kChunks], y[kTiles][2];
-  int64_t row[kTiles];
+  int64_t row[kTiles][2];
   const auto load_weights = [&](int set, int64_t n0) {
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
@@ -534,13 +534,14 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
   const auto load_y = [&](int t, int64_t n0) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int64_t n = n0 + 32 * half + 8 * g;
-      y[t][half] = load8_any<kWide>(a.y + row[t] * a.y_stride, n, a.features);
+      y[t][half] = load8_any<kWide>(a.y + row[t][half] * a.y_stride, n0 + (lane & 7) * 8, a.features);
     }
   };
   load_weights(0, place(0));
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) row[t] = a.order[tile.begin + min(t * 16 + m, tile.count - 1)];
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) row[t][half] = a.order[tile.begin + min(t * 16 + half * 8 + (lane >> 3), tile.count - 1)];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) load_y(t, place(0));
 
@@ -575,6 +576,8 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
     }
   }
 
+  float *turned = v + kTiles * 16 * kRow + wave * 16 * kTurned;
+  const uint32_t y_mask = a.has_y ? ~0u : 0u;
   const auto piece = [&](int set, int64_t n0, int64_t next) {
     load_weights(set ^ 1, next);
 #pragma unroll
@@ -591,26 +594,33 @@ __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapte
 #pragma unroll
           for (int f = 0; f < 4; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[set][f][c], lo[t][c], acc[f], 0, 0, 0);
         }
-#pragma unroll
-        for (int f = 0; f < 4; ++f) acc[f] *= back[t];
       }
+      // through LDS into the order of y: 8 lanes hold a row's 64 features, a line of memory each
+#pragma unroll
+      for (int f = 0; f < 4; ++f) *(float4_t *)(turned + m * kTurned + 32 * (f >> 1) + 8 * g + 4 * (f & 1)) = acc[f] * back[t];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
       half8_t r[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        const half8_t base = __builtin_bit_cast(half8_t, __builtin_bit_cast(uint4_t, y[t][half]) & y_mask);
+        const float *p = turned + (half * 8 + (lane >> 3)) * kTurned + (lane & 7) * 8;
+        const float4_t first4 = *(const float4_t *)p, second4 = *(const float4_t *)(p + 4);
         float sum[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)  // (tile 2 half + j / 4, row 4 g + j % 4 of the accumulators)
-          sum[j] = (a.has_y ? (float)y[t][half][j] : 0.f) + acc[2 * half + j / 4][j % 4];
+        for (int j = 0; j < 8; ++j) sum[j] = (float)base[j] + (j < 4 ? first4[j & 3] : second4[j & 3]);
         activate(sum, a.act);
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[half][j] = (half_t)sum[j];
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
       load_y(t, next);
-      if (t * 16 + m >= tile.count) continue;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int64_t n = n0 + 32 * half + 8 * g;
-        half_t *o = a.out + row[t] * a.out_stride + n;
+        if (t * 16 + half * 8 + (lane >> 3) >= tile.count) continue;
+        const int64_t n = n0 + (lane & 7) * 8;
+        half_t *o = a.out + row[t][half] * a.out_stride + n;
         if (kWide) {
           if (n < to) *(half8_t *)o = r[half];
         } else {
@@ -786,7 +796,7 @@ int start_down(const DownArgs &a, int64_t turns, hipStream_t stream) {
 
 template <int kRank, int kTiles, bool kWide>
 int start_up(const UpArgs &a, int64_t operands, hipStream_t stream) {
-  const size_t rows = (size_t)kTiles * 16 * (kRank + 4) * sizeof(float), operand = operands ? (size_t)2 * kRank * 72 * sizeof(half_t) : 0;
+  const size_t rows = (size_t)(kTiles * 16 * (kRank + 4) + kWaves * 16 * (64 + 4)) * sizeof(float), operand = operands ? (size_t)2 * kRank * 72 * sizeof(half_t) : 0;
   adapter_up_kernel<kRank, kTiles, kWide>
       <<<(unsigned)((int64_t)a.most_tiles * a.ranges + operands), kThreads, rows > operand ? rows : operand, stream>>>(a);
   return check_launch("adapter_up_kernel");
