@@ -334,43 +334,52 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
   const int wave_last = wave_row < rows ? s.first + (min(wave_row + kRowsOfWave, rows) - 1) / a.group : -1;
   const int group_last = s.first + (min(row0 + kRowsOfGroup, rows) - 1) / a.group;
   const int all_blocks = group_last < 0 ? 0 : group_last / kBlock + 1, share_of = (all_blocks + a.splits - 1) / a.splits;
-  const int first_block = min(all_blocks, (int)blockIdx.y * share_of), blocks = min(all_blocks, first_block + share_of);
+  const int first_block = min(all_blocks, (int)blockIdx.y * share_of), blocks = a.cache.n_blocks > 0 ? min(all_blocks, first_block + share_of) : 0;
 
   // staging: thread n has keys' piece (key, 16 dims c) and values' piece (dim d, 16 tokens)
+  static_assert(2 * kPieces == kDimTiles, "a piece for every dim tile of the result");
   uint4_t raw_k[kPieces], raw_v[kPieces];
   float ks = 0.f, vs = 0.f;  // of the block that is staged
   bool there = false;
+  int ahead = 0;  // the next block's id: it is asked for a block before its bytes are
+  const auto id_of = [&](int block) { return table[min(block, blocks - 1)]; };
+  // Loads are made without conditions, as in the adapters' products: of block 0 where an id is none, of other dims where a dim
+  // is behind the last (its queries are zeros, its results are not stored).
   const auto load = [&](int block) {
-    const int id = __builtin_amdgcn_readfirstlane(table[block]);
+    const int id = __builtin_amdgcn_readfirstlane(ahead);
     there = id >= 0 && id < a.cache.n_blocks;
-    if (!there) return;
-    const int64_t place = (int64_t)id * heads + h;
+    ahead = id_of(block + 1);
+    const int64_t place = (int64_t)(there ? id : 0) * heads + h;
     const uint8_t *kc = a.cache.k_codes + place * kBlock * dim, *vc = a.cache.v_codes + place * kBlock * dim;
     ks = a.cache.k_scale[place], vs = a.cache.v_scale[place];
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
       const int i = tid + n * kTileThreads, key = i / (DP / 16), c = i % (DP / 16), d = i / 4;
-      raw_k[n] = raw_v[n] = uint4_t{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};  // dims behind the last: zeros
-      if (c * 16 < dim) raw_k[n] = *(const uint4_t *)(kc + key * dim + c * 16);
-      if (d < dim) raw_v[n] = *(const uint4_t *)(vc + d * kBlock + i % 4 * 16);
+      raw_k[n] = *(const uint4_t *)(kc + key * dim + (c * 16 < dim ? c * 16 : 0));
+      raw_v[n] = *(const uint4_t *)(vc + (d < dim ? d : 0) * kBlock + i % 4 * 16);
     }
   };
   // Keys: operand (tile T, step c) is 1 KiB, lane (g, row) has dims 16 c + 8 g ...; a row's two halves are stored by the thread
   // that has its 16 dims.  The place within 512 bytes is turned by c, so that threads of one key and different c use
   // different banks.  Values: operand (dim tile, T, u), lane (g, dim) has tokens 32 T + 16 g + 8 u ...
-  const auto stage = [&](int buffer) {
+  const auto stage_piece = [&](int buffer, int n, bool values) {
     half_t *keys = tile_shared + buffer * 2 * kHalves, *vals = keys + kHalves;
-#pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
-      const int i = tid + n * kTileThreads, key = i / (DP / 16), c = i % (DP / 16), d = i / 4, piece = i % 4;
-      const int in_tile = key & 31, row = (in_tile >> 2 & 3) * 8 + (in_tile >> 4) * 4 + (in_tile & 3);
+    const int i = tid + n * kTileThreads;
+    if (!values) {
+      const int key = i / (DP / 16), c = i % (DP / 16), in_tile = key & 31, row = (in_tile >> 2 & 3) * 8 + (in_tile >> 4) * 4 + (in_tile & 3);
       half_t *to = keys + (((key >> 5) * kSteps + c) * 64 + (row ^ (c & 15))) * 8;
       store_codes(to, raw_k[n][0], raw_k[n][1]);
       store_codes(to + 32 * 8, raw_k[n][2], raw_k[n][3]);
-      half_t *tv = vals + (((d >> 5) * 4 + (piece >> 1) * 2) * 64 + (piece & 1) * 32 + (d & 31)) * 8;
-      store_codes(tv, raw_v[n][0], raw_v[n][1]);
-      store_codes(tv + 64 * 8, raw_v[n][2], raw_v[n][3]);
+    } else {
+      const int d = i / 4, piece = i % 4;
+      half_t *to = vals + (((d >> 5) * 4 + (piece >> 1) * 2) * 64 + (piece & 1) * 32 + (d & 31)) * 8;
+      store_codes(to, raw_v[n][0], raw_v[n][1]);
+      store_codes(to + 64 * 8, raw_v[n][2], raw_v[n][3]);
     }
+  };
+  const auto stage = [&](int buffer) {
+#pragma unroll
+    for (int n = 0; n < 2 * kPieces; ++n) stage_piece(buffer, n / 2, n & 1);
   };
 
   float16_t o[kDimTiles];
@@ -379,31 +388,35 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
 #pragma unroll
   for (int i = 0; i < kDimTiles; ++i) o[i] = float16_t{};
   if (first_block < blocks) {
+    ahead = id_of(first_block);
     load(first_block);
-    if (there) stage(first_block & 1);
+    stage(first_block & 1);
   }
-  bool fresh = true;
-  for (int block = first_block; block < blocks; ++block) {
-    __syncthreads();
-    const bool now = there;
-    // (not 0, which a masked score of -infinity would not survive: below 1e-30 every score is 0 to all that exp2 can tell)
-    float key_scale = ks * fabsf(a.scale_log2);
-    if (key_scale < 1e-30f) key_scale = 1e-30f;
-    const float value_scale = vs;
-    if (block + 1 < blocks) load(block + 1);
-    const int at = block * kBlock;
-    if (now && at <= wave_last) {
-      const half_t *keys = tile_shared + (block & 1) * 2 * kHalves, *vals = keys + kHalves;
-      // the value scale against its reference
-      if (value_scale > 0.f && value_scale < __builtin_inff() && (fresh || value_scale > 16.f * reference || value_scale * 16.f < reference)) {
-        const float turn = fresh ? 1.f : reference / value_scale;
-        reference = value_scale, fresh = false;
-        if (turn != 1.f) {
+  // Rescaling takes the accumulators out of the matrix units' registers and back, so it stands outside the loop over blocks,
+  // which leaves for it (before a block's probabilities) and comes back to the block: inside the loop, however seldom it ran, the
+  // compiler moved all of them for every block (2 x 2048 rows over 8000 keys, 16 heads of 256: 566 us).
+  bool fresh = true, again = false, now = false;
+  float keep = 1.f, key_scale = 1.f, value_scale = 0.f;
+  int block = first_block;
+  while (block < blocks) {
 #pragma unroll
-          for (int i = 0; i < kDimTiles; ++i) o[i] *= turn;
-        }
+    for (int i = 0; i < kDimTiles; ++i) o[i] *= keep;
+    for (; block < blocks; ++block, again = false) {
+      if (!again) {
+        __syncthreads();
+        now = there;
+        // (not 0, which a masked score of -infinity would not survive: below 1e-30 every score is 0 to all that exp2 can tell)
+        key_scale = ks * fabsf(a.scale_log2);
+        if (key_scale < 1e-30f) key_scale = 1e-30f;
+        value_scale = vs;
+        load(min(block + 1, blocks - 1));
       }
-      const float ratio = value_scale == 0.f ? 1.f : value_scale / reference;
+      const int at = block * kBlock;
+      if (!now || at > wave_last) {
+        stage((block + 1) & 1);
+        continue;
+      }
+      const half_t *keys = tile_shared + (block & 1) * 2 * kHalves, *vals = keys + kHalves;
       const bool masked = at + kBlock - 1 > wave_first;
       float16_t score[2];
 #pragma unroll
@@ -417,7 +430,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
       }
       // a row that sees none of this block takes nothing from it, also where its scales are not finite
       const bool none = at > position;
-      const float factor = none ? 1.f : key_scale, share = none ? 1.f : ratio;
+      const float factor = none ? 1.f : key_scale;
       float top = -__builtin_inff();
       if (masked) {
 #pragma unroll
@@ -432,14 +445,24 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
         for (int i = 0; i < 16; ++i) top = fmaxf(top, score[T][i]);
       top = fmaxf(top, __shfl_xor(top, 32)) * factor;
       const bool raise = top > most + 8.f || (most == -__builtin_inff() && top > most);
-      if (__any(raise)) {
+      // the value scale against its reference
+      const bool scaled = value_scale > 0.f && value_scale < __builtin_inff();
+      const bool turn = scaled && (fresh || value_scale > 16.f * reference || value_scale * 16.f < reference);
+      if (__builtin_expect(!again && (turn || __any(raise)), 0)) {
         const float next = raise ? top : most;
-        const float keep = raise ? __builtin_amdgcn_exp2f(most - next) : 1.f;
+        keep = raise ? __builtin_amdgcn_exp2f(most - next) : 1.f;
         most = next;
         sum *= keep;
-#pragma unroll
-        for (int i = 0; i < kDimTiles; ++i) o[i] *= keep;
+        if (turn) {
+          if (!fresh) keep *= reference / value_scale;
+          reference = value_scale, fresh = false;
+        }
+        if (block > first_block) {
+          again = true;
+          break;
+        }
       }
+      const float ratio = value_scale == 0.f ? 1.f : value_scale / reference, share = none ? 1.f : ratio;
       const float shift = __builtin_amdgcn_logf(share) - (most == -__builtin_inff() ? 0.f : most);
       half8_t pf[2][2];
       float part = 0.f;
@@ -452,19 +475,23 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
           pf[T][i >> 3][i & 7] = (half_t)p;
         }
       sum += part / share;
-      if (value_scale != 0.f) {  // (values of scale 0 are zeros, whatever their codes)
+      if (value_scale == 0.f) {  // (values of scale 0 are zeros, whatever their codes)
 #pragma unroll
-        for (int i = 0; i < kDimTiles; ++i)
+        for (int T = 0; T < 2; ++T) pf[T][0] = pf[T][1] = half8_t{};
+      }
 #pragma unroll
-          for (int T = 0; T < 2; ++T)
+      for (int i = 0; i < kDimTiles; ++i) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
-              o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
-            }
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
+          }
+        // (of bytes that are not there, or behind the last block, where nobody reads them)
+        stage_piece((block + 1) & 1, i / 2, i & 1);
       }
     }
-    if (block + 1 < blocks && there) stage((block + 1) & 1);
   }
   const float weight = sum + __shfl_xor(sum, 32);
   const int in_tile = wave * kRowsOfWave + m, row = row0 + in_tile;
