@@ -361,7 +361,8 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
   };
   // Keys: operand (tile T, step c) is 1 KiB, lane (g, row) has dims 16 c + 8 g ...; a row's two halves are stored by the thread
   // that has its 16 dims.  The place within 512 bytes is turned by c, so that threads of one key and different c use
-  // different banks.  Values: operand (dim tile, T, u), lane (g, dim) has tokens 32 T + 16 g + 8 u ...
+  // different banks.  Values: operand (dim tile, T, u), lane (g, dim) has tokens 32 T + 16 g + 8 u ..., turned by the piece for the
+  // same reason (four threads of a dim would write to one bank).
   const auto stage_piece = [&](int buffer, int n, bool values) {
     half_t *keys = tile_shared + buffer * 2 * kHalves, *vals = keys + kHalves;
     const int i = tid + n * kTileThreads;
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
       store_codes(to + 32 * 8, raw_k[n][2], raw_k[n][3]);
     } else {
       const int d = i / 4, piece = i % 4;
-      half_t *to = vals + (((d >> 5) * 4 + (piece >> 1) * 2) * 64 + (piece & 1) * 32 + (d & 31)) * 8;
+      half_t *to = vals + (((d >> 5) * 4 + (piece >> 1) * 2) * 64 + (piece & 1) * 32 + ((d & 31) ^ (2 * piece))) * 8;
       store_codes(to, raw_v[n][0], raw_v[n][1]);
       store_codes(to + 64 * 8, raw_v[n][2], raw_v[n][3]);
     }
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
         for (int T = 0; T < 2; ++T)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + lane) * 8);
+            const half8_t vf = *(const half8_t *)(vals + (((i * 2 + T) * 2 + u) * 64 + g * 32 + (m ^ (2 * (2 * T + g)))) * 8);
             o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[T][u], o[i], 0, 0, 0);
           }
         // (of bytes that are not there, or behind the last block, where nobody reads them)
