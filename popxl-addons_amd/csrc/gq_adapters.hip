@@ -767,9 +767,13 @@ int64_t down_splits(int64_t tiles, int64_t features) {
   return want < most ? want : most > 0 ? most : 1;
 }
 
-// Rows of a tile: 16 for decode batches, whose rows mostly have adapters of their own; 64 where an adapter's weights are worth
-// reading once for more rows.
-bool large_tiles(int64_t rows) { return rows >= 1024; }
+// Rows of a tile: 16 for decode batches, whose rows mostly have adapters of their own, and as long as tiles of 64 would not
+// fill the device; 64 where an adapter's weights are worth reading once for more rows, the sooner the higher the rank (but ranks
+// above 64 leave tiles of 64 rows one wave a SIMD).  Projection with 8 adapters, 4096 features to 4096 (* to 12288), us with
+// tiles of 16 and 64: rank 16, rows 1024: 17 and 20, 4096: 34 and 43, 8192*: 130 and 126, rank 32, 32768: 229 and 209;
+// rank 64, rows 512: 23 and 23, 1024: 31 and 28, 8192: 118 and 91; rank 128, rows 2048*: 121 and 134, 4096*: 196 and 181,
+// 8192: 198 and 169.
+bool large_tiles(int64_t rows, int64_t rank) { return rows >= (rank <= 32 ? 8192 : rank <= 64 ? 1024 : 4096); }
 
 struct Batch {
   const PlanLayout plan;
@@ -881,7 +885,7 @@ struct GradLayout {
   }
 };
 
-int64_t tiles_at_most(const PlanLayout &plan) { return large_tiles(plan.rows) ? plan.most_large : plan.most_small; }
+int64_t tiles_at_most(const PlanLayout &plan, int64_t rank) { return large_tiles(plan.rows, rank) ? plan.most_large : plan.most_small; }
 
 }  // namespace
 
@@ -898,12 +902,12 @@ int launch_adapter_plan(const int32_t *ids, int64_t rows, int64_t adapters, void
 
 int64_t adapter_apply_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t rank) {
   const PlanLayout plan(rows, adapters);
-  return round_up(down_splits(tiles_at_most(plan), in) * rows * rank_class(rank) * 4, 256);
+  return round_up(down_splits(tiles_at_most(plan, rank), in) * rows * rank_class(rank) * 4, 256);
 }
 
 int launch_adapter_apply(const gq_adapters &w, const void *plan, int64_t rows, const uint16_t *x, int64_t x_stride, const uint16_t *y,
                          int64_t y_stride, uint16_t *out, int64_t out_stride, int act, void *workspace, hipStream_t stream) {
-  const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows)};
+  const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows, w.rank)};
   const int64_t splits = down_splits(b.most_tiles(), w.in_features);
   const int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, w.in_features, w.rank, (float *)workspace, nullptr, splits, nullptr, stream);
   if (rc != GQ_OK) return rc;
@@ -913,14 +917,14 @@ int launch_adapter_apply(const gq_adapters &w, const void *plan, int64_t rows, c
 
 int64_t adapter_grad_workspace_bytes(int64_t rows, int64_t adapters, int64_t in, int64_t out, int64_t rank) {
   const PlanLayout plan(rows, adapters);
-  const int64_t tiles = tiles_at_most(plan);
+  const int64_t tiles = tiles_at_most(plan, rank);
   return GradLayout(plan, tiles, in, out, rank, down_splits(tiles, in), down_splits(tiles, out)).bytes;
 }
 
 int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, const uint16_t *x, int64_t x_stride, const uint16_t *dy,
                         int64_t dy_stride, const uint16_t *dx, int64_t dx_stride, uint16_t *dx_out, int64_t dx_out_stride, float *d_down,
                         float *d_up, void *workspace, hipStream_t stream) {
-  const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows)};
+  const Batch b = {PlanLayout(rows, w.n_adapters), (const int *)plan, large_tiles(rows, w.rank)};
   const int64_t in = w.in_features, out = w.out_features, tiles = b.most_tiles();
   const int64_t in_splits = down_splits(tiles, in), out_splits = down_splits(tiles, out);
   const GradLayout l(b.plan, tiles, in, out, w.rank, in_splits, out_splits);

@@ -38,6 +38,10 @@ SIZES = [  # rows, in, out, rank, adapters
     (1500, 96, 100, 24, 7),
     (1100, 136, 200, 100, 2),
     (2048, 64, 72, 5, 1),
+    (1030, 264, 72, 64, 2),
+    (4100, 72, 136, 100, 3),
+    (8193, 72, 80, 16, 2),
+    (8200, 40, 33, 20, 1),
 ]
 
 
