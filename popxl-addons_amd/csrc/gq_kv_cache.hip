@@ -11,7 +11,7 @@
 // scale is a maximum over all of it, and no other workgroup writes there.  The new tokens come by 16-byte loads that are
 // contiguous over a row and wait in LDS, as binary16, for the scale; from there key codes go out 8 dims at a time, and value
 // codes, which the cache holds transposed, 16 tokens of a dim at a time.  Keys that are turned on the way: the angles of the
-// block's tokens are formed once in LDS and serve several heads.  (With the tokens held in registers instead the kernel had 160
+// block's tokens are formed once in LDS.  (With the tokens held in registers instead the kernel had 160
 // of them and 23 KiB of code, and a decode step waited for its instructions: 19 us for 48 requests.)
 #include "gq_kv.h"
 #include "gq_rotary.h"
@@ -20,6 +20,7 @@ namespace gq {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kFewOfBlock = 4;  // new tokens of a sequence, on average, up to which a workgroup is one wave
 constexpr int kFew = 8;  // new tokens of a block up to which their value codes are stored byte by byte
 
 struct AppendArgs {
@@ -29,7 +30,7 @@ struct AppendArgs {
   int64_t token[2], head[2];
   const double *turns;  // NULL: keys are stored as they come
   float factor;
-  int rotary_dim, heads_per_group;
+  int rotary_dim;
   int first;  // blockIdx.y + first: 0 keys, 1 values
   bool half_layout;
 };
@@ -111,16 +112,16 @@ template <int kSize>
 __global__ __launch_bounds__(kSize) void kv_append_kernel(AppendArgs a) {
   constexpr int kAhead = 4;
   extern __shared__ uint4_t append_shared[];  // rows: binary16 [token][dim]; turn: cosine and sine [token][pair]
-  __shared__ uint32_t wave_max[2][kSize / 64];
+  __shared__ uint32_t wave_max[kSize / 64];
   const int tid = threadIdx.x;
   const bool values = blockIdx.y + a.first != 0;
   // (heads run fastest: the workgroups under way together then cover whole rows of the tokens, not one head's stretch of each)
-  const int dim = a.cache.dim, columns = dim / 8, heads = a.cache.heads, groups = (heads + a.heads_per_group - 1) / a.heads_per_group;
+  const int dim = a.cache.dim, columns = dim / 8, heads = a.cache.heads, h = blockIdx.x % heads;
   Place p;
-  if (!find_place(a.cache, a.batch, blockIdx.x / groups, p)) return;
+  if (!find_place(a.cache, a.batch, blockIdx.x / heads, p)) return;
   const int rotary_dim = values || !a.turns ? 0 : a.rotary_dim, pairs = rotary_dim / 2;
-  const half_t *from = (values ? a.x[1] : a.x[0]) + p.row * (values ? a.token[1] : a.token[0]);
-  const int64_t stride = values ? a.token[1] : a.token[0], head_stride = values ? a.head[1] : a.head[0];
+  const int64_t stride = values ? a.token[1] : a.token[0], place = (int64_t)p.id * heads + h;
+  const half_t *x = (values ? a.x[1] : a.x[0]) + p.row * stride + h * (values ? a.head[1] : a.head[0]);
   half_t *rows = (half_t *)append_shared;
   float2 *turn = (float2 *)(rows + p.count * dim);
   const int twos = a.half_layout ? pairs / 8 : 0, per_token = columns - twos;  // (half layout: units of two pieces)
@@ -139,138 +140,130 @@ __global__ __launch_bounds__(kSize) void kv_append_kernel(AppendArgs a) {
     }
   }
 
-  const int h0 = blockIdx.x % groups * a.heads_per_group, h1 = min(heads, h0 + a.heads_per_group);
-  for (int h = h0; h < h1; ++h) {
-    const int64_t place = (int64_t)p.id * heads + h;
-    const half_t *x = from + h * head_stride;
-    float *scale_at = (values ? a.cache.v_scale : a.cache.k_scale) + place;
-    const float old = p.slot > 0 ? *scale_at : 0.f;
-    if (rotary_dim > 0 && h == h0) __syncthreads();  // (the angles are there)
-    uint32_t most = 0;  // the largest magnitudes, as two 16-bit patterns: NaN above infinity above all numbers
-    const auto put = [&](int token, int d, half8_t w) {
-      most = magnitudes(w, most);
-      *(half8_t *)(rows + token * dim + d) = w;
-    };
-    for (int n0 = tid; n0 < units; n0 += kAhead * kSize) {
-      half8_t v[kAhead], other[kAhead];
+  float *scale_at = (values ? a.cache.v_scale : a.cache.k_scale) + place;
+  const float old = p.slot > 0 ? *scale_at : 0.f;
+  if (rotary_dim > 0) __syncthreads();  // (the angles are there)
+  uint32_t most = 0;  // the largest magnitudes, as two 16-bit patterns: NaN above infinity above all numbers
+  const auto put = [&](int token, int d, half8_t w) {
+    most = magnitudes(w, most);
+    *(half8_t *)(rows + token * dim + d) = w;
+  };
+  for (int n0 = tid; n0 < units; n0 += kAhead * kSize) {
+    half8_t v[kAhead], other[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int n = n0 + i * kSize, token = n * per_unit >> 16, u = n - token * per_token;
-        v[i] = other[i] = half8_t{};
-        if (n >= units) continue;
-        // a unit is 8 dims, or, among the first of a token, 8 dims and those they are turned with
-        v[i] = *(const half8_t *)(x + token * stride + (u < twos ? u : u + twos) * 8);
-        if (u < twos) other[i] = *(const half8_t *)(x + token * stride + pairs + u * 8);
-      }
+    for (int i = 0; i < kAhead; ++i) {
+      // a unit is 8 dims, or, among the first of a token, 8 dims and those they are turned with (the last unit again behind it)
+      const int n = min(n0 + i * kSize, units - 1), token = n * per_unit >> 16, u = n - token * per_token;
+      v[i] = *(const half8_t *)(x + token * stride + (u < twos ? u : u + twos) * 8);
+      if (twos > 0) other[i] = *(const half8_t *)(x + token * stride + (u < twos ? pairs + u * 8 : 0));
+    }
 #pragma unroll 1
-      for (int i = 0; i < kAhead; ++i) {
-        const int n = n0 + i * kSize, token = n * per_unit >> 16, u = n - token * per_token;
-        if (n >= units) break;
-        half8_t w = v[0];
-        if (u < twos) {
-          half8_t w2;
-          const float2 *cs = turn + token * pairs + u;
+    for (int i = 0; i < kAhead; ++i) {
+      const int n = n0 + i * kSize, token = n * per_unit >> 16, u = n - token * per_token;
+      if (n >= units) break;
+      half8_t w = v[0];
+      if (u < twos) {
+        half8_t w2;
+        const float2 *cs = turn + token * pairs + u;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            half_t lo, hi;
-            rotary_pair((float)w[j], (float)other[0][j], cs[j * stretch], lo, hi);
-            w[j] = lo, w2[j] = hi;
-          }
-          put(token, pairs + u * 8, w2);
-        } else if (twos == 0 && u * 8 < rotary_dim) {
-          const float2 *cs = turn + token * pairs + u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            half_t lo, hi;
-            rotary_pair((float)w[2 * j], (float)w[2 * j + 1], cs[j * stretch], lo, hi);
-            w[2 * j] = lo, w[2 * j + 1] = hi;
-          }
+        for (int j = 0; j < 8; ++j) {
+          half_t lo, hi;
+          rotary_pair((float)w[j], (float)other[0][j], cs[j * stretch], lo, hi);
+          w[j] = lo, w2[j] = hi;
         }
-        put(token, (u < twos ? u : u + twos) * 8, w);
+        put(token, pairs + u * 8, w2);
+      } else if (twos == 0 && u * 8 < rotary_dim) {
+        const float2 *cs = turn + token * pairs + u;
 #pragma unroll
-        for (int k = 0; k + 1 < kAhead; ++k) v[k] = v[k + 1], other[k] = other[k + 1];  // (one copy of this code for the four)
+        for (int j = 0; j < 4; ++j) {
+          half_t lo, hi;
+          rotary_pair((float)w[2 * j], (float)w[2 * j + 1], cs[j * stretch], lo, hi);
+          w[2 * j] = lo, w[2 * j + 1] = hi;
+        }
       }
-    }
-    most = max(most & 0xffff, most >> 16);
+      put(token, (u < twos ? u : u + twos) * 8, w);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-    if ((tid & 63) == 0) wave_max[h & 1][tid >> 6] = most;
-    __syncthreads();  // (every thread has read the old scale, too)
-#pragma unroll
-    for (int w = 0; w < kSize / 64; ++w) most = max(most, wave_max[h & 1][w]);
-    const float need = (float)__builtin_bit_cast(half_t, (uint16_t)most) / 127.f;  // infinite or NaN where an input is
-    float scale = old, shrink = 1.f;
-    if (!(need <= old) && old == old) {  // (a scale that is NaN stays)
-      scale = need;
-      if (old > 0.f && need < __builtin_inff()) {
-        int e;
-        if (frexpf(need / old, &e) == 0.5f) --e;
-        scale = ldexpf(old, e);
-        shrink = ldexpf(1.f, -e);
-      }
+      for (int k = 0; k + 1 < kAhead; ++k) v[k] = v[k + 1], other[k] = other[k + 1];  // (one copy of this code for the four)
     }
-    if (tid == 0 && (scale != old || p.slot == 0)) *scale_at = scale;
+  }
+  most = max(most & 0xffff, most >> 16);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+  if ((tid & 63) == 0) wave_max[tid >> 6] = most;
+  __syncthreads();  // (every thread has read the old scale, too)
+#pragma unroll
+  for (int w = 0; w < kSize / 64; ++w) most = max(most, wave_max[w]);
+  const float need = (float)__builtin_bit_cast(half_t, (uint16_t)most) / 127.f;  // infinite or NaN where an input is
+  float scale = old, shrink = 1.f;
+  if (!(need <= old) && old == old) {  // (a scale that is NaN stays)
+    scale = need;
+    if (old > 0.f && need < __builtin_inff()) {
+      int e;
+      if (frexpf(need / old, &e) == 0.5f) --e;
+      scale = ldexpf(old, e);
+      shrink = ldexpf(1.f, -e);
+    }
+  }
+  if (tid == 0 && (scale != old || p.slot == 0)) *scale_at = scale;
 
-    uint8_t *codes = (values ? a.cache.v_codes : a.cache.k_codes) + place * kBlock * dim;
-    if (shrink != 1.f) {  // tokens that were there: slots [0, slot)
-      for (int n = tid; n < (values ? dim * 16 : p.slot * dim / 4); n += kSize) {
-        const int t0 = values ? n % 16 * 4 : 0;
-        if (values && t0 >= p.slot) continue;
-        const uint32_t w = ((uint32_t *)codes)[n], keep = values && t0 + 4 > p.slot ? 0xffffffffu << 8 * (p.slot - t0) : 0u;
-        ((uint32_t *)codes)[n] = (scaled_down(w, shrink) & ~keep) | (w & keep);
-      }
-      if (values) __syncthreads();  // (a word may hold bytes of new tokens too, stored below)
+  uint8_t *codes = (values ? a.cache.v_codes : a.cache.k_codes) + place * kBlock * dim;
+  if (shrink != 1.f) {  // tokens that were there: slots [0, slot)
+    for (int n = tid; n < (values ? dim * 16 : p.slot * dim / 4); n += kSize) {
+      const int t0 = values ? n % 16 * 4 : 0;
+      if (values && t0 >= p.slot) continue;
+      const uint32_t w = ((uint32_t *)codes)[n], keep = values && t0 + 4 > p.slot ? 0xffffffffu << 8 * (p.slot - t0) : 0u;
+      ((uint32_t *)codes)[n] = (scaled_down(w, shrink) & ~keep) | (w & keep);
     }
+    if (values) __syncthreads();  // (a word may hold bytes of new tokens too, stored below)
+  }
 
-    const Coder code(scale);
-    if (!values || p.count < kFew) {
+  const Coder code(scale);
+  if (!values || p.count < kFew) {
 #pragma unroll 2
-      for (int n = tid; n < p.count * columns; n += kSize) {
-        const int token = n * per_column >> 16, c = n - token * columns;
-        const half8_t v = *(const half8_t *)(rows + token * dim + c * 8);
-        const uint2_t w = code(v);
-        if (!values) {
-          *(uint2_t *)(codes + (p.slot + token) * dim + c * 8) = w;
-        } else {
+    for (int n = tid; n < p.count * columns; n += kSize) {
+      const int token = n * per_column >> 16, c = n - token * columns;
+      const half8_t v = *(const half8_t *)(rows + token * dim + c * 8);
+      const uint2_t w = code(v);
+      if (!values) {
+        *(uint2_t *)(codes + (p.slot + token) * dim + c * 8) = w;
+      } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) codes[(c * 8 + j) * kBlock + p.slot + token] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
-        }
+        for (int j = 0; j < 8; ++j) codes[(c * 8 + j) * kBlock + p.slot + token] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
       }
-    } else {
-      for (int n = tid; n < dim * 2; n += kSize) {  // two dims, 16 slots
-        const int d = n / 4 * 2, t0 = n % 4 * 16;  // (a row's 64 bytes by four lanes)
-        if (t0 + 15 < p.slot || t0 >= end) continue;
-        const half_t *column = rows + (t0 - p.slot) * dim + d;
-        uint4_t w[2];
+    }
+  } else {
+    for (int n = tid; n < dim * 2; n += kSize) {  // two dims, 16 slots
+      const int d = n / 4 * 2, t0 = n % 4 * 16;  // (a row's 64 bytes by four lanes)
+      if (t0 + 15 < p.slot || t0 >= end) continue;
+      const half_t *column = rows + (t0 - p.slot) * dim + d;
+      uint4_t w[2];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {  // 8 slots
-          half8_t v[2];
+      for (int q = 0; q < 2; ++q) {  // 8 slots
+        half8_t v[2];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const half2_t two = *(const half2_t *)(column + (min(max(t0 + 8 * q + i, p.slot), end - 1) - t0) * dim);
-            v[0][i] = two[0], v[1][i] = two[1];
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint2_t eight = code(v[i]);
-            w[i][2 * q] = eight[0], w[i][2 * q + 1] = eight[1];
-          }
+        for (int i = 0; i < 8; ++i) {
+          const half2_t two = *(const half2_t *)(column + (min(max(t0 + 8 * q + i, p.slot), end - 1) - t0) * dim);
+          v[0][i] = two[0], v[1][i] = two[1];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint8_t *to = codes + (d + i) * kBlock + t0;
-          if (t0 >= p.slot && t0 + 16 <= end) {
-            *(uint4_t *)to = w[i];
-          } else {
-            for (int j = max(p.slot - t0, 0); j < min(end - t0, 16); ++j) {
-              const uint32_t word = j < 4 ? w[i][0] : j < 8 ? w[i][1] : j < 12 ? w[i][2] : w[i][3];
-              to[j] = (uint8_t)(word >> 8 * (j & 3));
-            }
+          const uint2_t eight = code(v[i]);
+          w[i][2 * q] = eight[0], w[i][2 * q + 1] = eight[1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint8_t *to = codes + (d + i) * kBlock + t0;
+        if (t0 >= p.slot && t0 + 16 <= end) {
+          *(uint4_t *)to = w[i];
+        } else {
+          for (int j = max(p.slot - t0, 0); j < min(end - t0, 16); ++j) {
+            const uint32_t word = j < 4 ? w[i][0] : j < 8 ? w[i][1] : j < 12 ? w[i][2] : w[i][3];
+            to[j] = (uint8_t)(word >> 8 * (j & 3));
           }
         }
       }
     }
-    __syncthreads();  // (the next head's rows)
   }
 }
 
@@ -354,19 +347,19 @@ int launch_kv_append(const KvCache &cache, const KvBatch &batch, const uint16_t 
   const int64_t places = most_places(batch);
   const int rows = batch.tokens < kBlock ? batch.tokens : kBlock;
   const size_t codes = (size_t)rows * cache.dim * sizeof(half_t), angles = rotary ? (size_t)rows * rotary->rotary_dim / 2 * sizeof(float2) : 0;
-  if (batch.tokens < kFew * batch.sequences) {
-    a.heads_per_group = 1;
+  // Blocks of few tokens: one wave each (48 sequences of 1, about 2, about 4 tokens, 16 heads of 256: 11, 15, 27 us, with four waves
+  // 14, 17, 21; 8 sequences of 1, about 8 tokens, 8 heads of 128: 5.5 and 11, with four waves 10 and 12).
+  if (batch.tokens < kFewOfBlock * batch.sequences) {
     if (const int rc = allow_lds((const void *)kv_append_kernel<64>, codes + angles)) return rc;
     kv_append_kernel<64><<<dim3((unsigned)(places * cache.heads), 2), 64, codes + angles, stream>>>(a);
   } else {
-    // Keys and values apart: the angles take as much LDS as the rows or twice that, which only the keys' workgroups need.  They
-    // are worth sharing between heads where there are workgroups enough anyway, as is what every workgroup does first.
+    // Keys and values apart: the angles take as much LDS as the rows or twice that, which only the keys' workgroups need.
+    // (Sharing the angles between four heads of a workgroup took 47 us where this takes 43, for 16383 tokens, 8 heads of 128, and
+    // 45 where this takes 28, for 48 sequences of about 8 tokens, 16 heads of 256.)
     if (const int rc = allow_lds((const void *)kv_append_kernel<kThreads>, codes + angles)) return rc;
-    a.heads_per_group = places * cache.heads >= 1536 ? 4 : 1;
-    const int groups = (cache.heads + a.heads_per_group - 1) / a.heads_per_group;
-    kv_append_kernel<kThreads><<<(unsigned)(places * groups), kThreads, codes + angles, stream>>>(a);
+    kv_append_kernel<kThreads><<<(unsigned)(places * cache.heads), kThreads, codes + angles, stream>>>(a);
     a.first = 1;
-    kv_append_kernel<kThreads><<<(unsigned)(places * groups), kThreads, codes, stream>>>(a);
+    kv_append_kernel<kThreads><<<(unsigned)(places * cache.heads), kThreads, codes, stream>>>(a);
   }
   return check_launch("kv_append_kernel");
 }
