@@ -761,10 +761,20 @@ __global__ __launch_bounds__(kThreads) void adapter_sum_kernel(OuterArgs a) {
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int rank_class(int64_t rank) { return rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
-// Workgroups that fill the device twice over where the features allow it, each with at least 512 features (128 a wave)
+// Workgroups that fill the device twice over where the features allow it, each with at least 512 features (128 a wave).  With
+// once, twice, four times as many: 31, 25, 32 us (6001 rows of 4096, rank 32), 127, 79, 81 us (8192 rows of 16384, rank 64).
 int64_t down_splits(int64_t tiles, int64_t features) {
   const int64_t most = (features + 511) / 512, want = (512 + tiles - 1) / tiles;
   return want < most ? want : most > 0 ? most : 1;
+}
+
+// As many workgroups as are resident together, no more: each sums its tile's v anew, and a few behind the others cost as much as
+// a whole turn of them (6001 rows to 12288, rank 32, 376 tiles: 2, 3, 6 ranges 74, 80, 77 us; 8192 rows to 4096, rank 64, 128
+// tiles: 4, 8 ranges 43, 52 us; 150 rows to 16384, rank 64: 13, 16, 32 ranges 27, 24, 29 us).  `tiles` counts
+// the last one of every adapter: an eighth of them may be nobody's.
+int64_t up_ranges(int64_t tiles, int64_t rank, bool large) {
+  const int64_t resident = large || rank > 64 ? 512 : 1024, ranges = (resident + tiles / 8) / tiles;
+  return ranges > 0 ? ranges : 1;
 }
 
 // Rows of a tile: 16 for decode batches, whose rows mostly have adapters of their own, and as long as tiles of 64 would not
@@ -837,8 +847,8 @@ int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, c
   a.tiles = b.tiles(), a.tile_count = b.words + b.plan.counts + (b.large ? 1 : 0), a.order = b.words + b.plan.order;
   a.rows = b.plan.rows, a.features = features, a.rank = (int)rank, a.splits = (int)splits, a.act = act;
   a.skip_rows_without = y == out && y_stride == out_stride && act == GQ_ACT_NONE;
-  const int64_t tiles = b.most_tiles(), most = (features + 255) / 256, want = (1024 + tiles - 1) / tiles;
-  a.range = round_up((features + (want < most ? want : most) - 1) / (want < most ? want : most), 256);
+  const int64_t tiles = b.most_tiles(), most = (features + 255) / 256, want = up_ranges(tiles, rank, b.large), ranges = want < most ? want : most;
+  a.range = round_up((features + ranges - 1) / ranges, 256);
   a.most_tiles = (int)tiles, a.ranges = (int)((features + a.range - 1) / a.range);
   if (outer) a.outer = *outer;
   const int64_t longest = b.plan.rows < kAdapterSegment ? b.plan.rows : kAdapterSegment;
