@@ -443,7 +443,7 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
  * A batch is B sequences.  Rows offsets[b] ... offsets[b + 1] - 1 of the row tensors (k, v, q, out) are the newest tokens of
  * sequence b, seq_lens[b] its length with them: its last row has position seq_lens[b] - 1.  A sequence that is given more rows
  * than it has tokens is padded in front: those rows are not stored and attend to nothing (zeros).  Token t of sequence b lies in
- * block block_table[b][t / GQ_KV_BLOCK]; no two sequences of a batch may append to the same block.  offsets ascend from 0;
+ * block block_table[b][t / GQ_KV_BLOCK]; a batch may append to a block at one place of its table only.  offsets ascend from 0;
  * rows from offsets[B] on are neither read nor written.  These arrays are device data that no call waits for: a length beyond
  * the table's width is cut to it, and a block number outside [0, n_blocks) is a block that is not there -- nothing is stored
  * in it, nothing read back from it, and attention passes over its tokens.
@@ -456,7 +456,7 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
  * gq_kv_gather_f16     the values of the batch's rows, [tokens, kv_heads, head_dim] binary16, contiguous, 16-byte aligned.
  * gq_kv_attention_f16  out[row][head] = softmax(scale q . k) v over the tokens at the row's position and before, query head i
  *   with kv head i / (q_heads / kv_heads).  q, out [tokens, q_heads, head_dim]: q strides multiples of 8 and 16-byte aligned,
- *   out any strides (elements).  Binary32 softmax and sums; probabilities enter the product with the values as binary16.
+ *   out any strides (elements), apart from q.  Binary32 softmax and sums; probabilities enter the product with the values as binary16.
  *   workspace: gq_kv_attention_workspace_bytes() bytes, 16-byte aligned, any contents, not shared by calls that may overlap.
  */
 #define GQ_KV_BLOCK 64
@@ -494,7 +494,7 @@ int gq_kv_attention_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, cons
  * gq_adapter_apply_f16   x [rows, in], y and out [rows, out] (row strides in elements; y == NULL: zeros; out may be y with the
  *   same stride).  The fast kernels need 16-byte aligned rows and rank % 8 == 0.
  * gq_adapter_grad_f16    from dy = dL/dout (no activation): dx_out = dx + scaling dy up down (dx == NULL: zeros; dx_out may be
- *   dx with the same stride), d_down [n_adapters, rank, in] and d_up [n_adapters, out, rank] in binary32, zeros for
+ *   dx with the same stride, and lies apart from x and dy), d_down [n_adapters, rank, in] and d_up [n_adapters, out, rank] in binary32, zeros for
  *   adapters without rows.
  * Each workspace: the matching size function's bytes, 256-byte aligned, any contents, not shared by calls that may overlap.
  * The order of every sum is fixed by the sizes and ids: equal calls give equal bits.

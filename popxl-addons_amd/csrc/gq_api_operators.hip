@@ -244,6 +244,8 @@ int gq_adapter_grad_f16(const gq_adapters *adapters, const void *plan, int64_t r
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: a stride is negative or exceeds 2^30", who);
   if (dx == dx_out && dx_row_stride != dx_out_row_stride)
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: in place, dx and dx_out must have the same stride", who);
+  if (dx_out == x || dx_out == dy)  // (both are read again behind it)
+    return gq::fail(GQ_ERR_UNSUPPORTED, "%s: dx_out must not be x or dy", who);
   rc = gq::check_workspace(who, workspace, workspace_bytes,
                            gq::adapter_grad_workspace_bytes(rows, adapters->n_adapters, adapters->in_features, adapters->out_features,
                                                             adapters->rank), 256);

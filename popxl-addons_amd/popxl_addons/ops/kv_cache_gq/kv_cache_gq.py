@@ -9,7 +9,8 @@ A batch is described by three int32 tensors on the device, which no call waits f
     block_table [B, W]   token t of sequence b lies in block block_table[b, t // BLOCK_SIZE] of the cache
 A sequence with more rows than tokens is padded in front: those rows are not stored and attend to nothing (zeros).  Rows from
 offsets[B] on are neither read nor written.  A block number outside the cache is a block that is not there: nothing is stored in
-it and attention passes over its tokens.  Two sequences may read the same block; only one of a batch may append to it.
+it and attention passes over its tokens.  Two sequences may read the same block; a batch may append to it at one place of the
+table only.
 """
 import ctypes
 
@@ -168,7 +169,8 @@ def kv_cache_attention(q, cache, offsets, seq_lens, block_table, scale=None, out
             i // (q_heads / kv_heads)
         offsets, seq_lens, block_table: the batch (see the module)
         scale (float): of the scores, head_dim ** -0.5 if None
-        out (torch.Tensor): float16, the shape of q; a new tensor if None, whose rows from offsets[B] on hold nothing in particular
+        out (torch.Tensor): float16, the shape of q, apart from it; a new tensor if None, whose rows from offsets[B] on hold
+            nothing in particular
 
     Returns:
         torch.Tensor: `out`.  Decode steps, prompts in chunks and mixtures of both are one call; results do not depend on timing.

@@ -173,6 +173,14 @@ def test_adapter_refusals():
     _gq_hip.call("gq_adapter_plan", 0, 0, 4, 0, 0, None)
 
 
+@pytest.mark.parametrize("x,dy", [(64, 16), (16, 64)])
+def test_adapter_gradient_apart_from_what_it_reads(x, dy):
+    """dx_out is written before the gradients of the weights read x and dy."""
+    a = _gq_hip.Adapters(16, 16, 16, 4, 8, 64, 64)
+    message = _refused(GQ_ERR_UNSUPPORTED, "gq_adapter_grad_f16", _address(a), 16, 5, x, 64, dy, 64, 32, 64, 64, 64, 16, 16, 256, 1 << 40, None)
+    assert "dx_out must not be x or dy" in message
+
+
 def test_frequencies():
     w, factor = rotary_frequencies(64)
     assert factor == 1 and w[0] == 1 and w.shape == (32,) and math.isclose(w[-1], 10000 ** (-62 / 64))
