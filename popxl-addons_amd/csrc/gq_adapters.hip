@@ -5,7 +5,7 @@
 //                      adapter, so that each product below is a plain matrix product over gathered rows.
 // adapter_down_kernel  v = x A^T (contraction over the features): a split of the features per workgroup, binary32 parts.
 // adapter_up_kernel    y' = act(y + s v B^T) (contraction over the rank).
-//   The gradients are the same two products with the weights turned (adapter_turn_kernel): dv = dy B, dx' = dx + s dv A, and
+//   The gradients are the same two products with the weights turned (turn_weights): dv = dy B, dx' = dx + s dv A, and
 // adapter_outer_kernel dA = s dv^T x, dB = s dy^T v (contraction over rows; parts of 2048 rows, added in order by
 //                      adapter_sum_kernel; no atomics anywhere, so results do not depend on timing).
 //
@@ -14,6 +14,10 @@
 // contraction over no more than 128.
 //
 // Bound by memory: x, y, y' and the adapters in use, each once; ranks of 8 ... 64 give 2 rank flops a byte of x.
+//
+// Measured (TB/s of rows): 6001 rows, 4096 to 12288, rank 32: adapter_down_kernel 23 us (2.1), adapter_up_kernel 73 us (4.0).
+// Gradients of 8192 rows, 4096 to 16384, rank 64: x A^T 28 us (2.4, the turned weights with it), dy B 77 us (3.5), dx 42 us
+// (3.2, the operands with it), the outer products 105 us (3.2), their sum 9 us.  A decode batch of 8 rows: 4 and 4.4 us, two launches.
 #include "gq_adapters.h"
 
 namespace gq {
@@ -41,8 +45,30 @@ __device__ __forceinline__ uint64_t same_kind(int kind, bool valid) {
   return mask;
 }
 
-// One workgroup.  Wave w takes the w-th stretch of rows: it counts them by kind (adapter, or none = the last kind), a scan over
-// kinds and waves gives every (kind, wave) its place, and the wave puts its rows there in their order.
+// An adapter's rows in the lists of tiles and segments.
+struct Listed {
+  int adapter, rows, begin, small, large, segment, part;
+};
+
+__device__ __forceinline__ void list(const PlanArgs &a, const Listed &l, int first, int step) {
+  for (int i = first; i * kAdapterSmallTile < l.rows; i += step)
+    ((AdapterTile *)(a.plan + a.small))[l.small + i] =
+        AdapterTile{l.adapter, l.begin + i * kAdapterSmallTile, min(l.rows - i * kAdapterSmallTile, kAdapterSmallTile)};
+  for (int i = first; i * kAdapterLargeTile < l.rows; i += step)
+    ((AdapterTile *)(a.plan + a.large))[l.large + i] =
+        AdapterTile{l.adapter, l.begin + i * kAdapterLargeTile, min(l.rows - i * kAdapterLargeTile, kAdapterLargeTile)};
+  if (l.adapter < 0) return;
+  for (int i = first; i * kAdapterSegment < l.rows; i += step)
+    ((AdapterTile *)(a.plan + a.segments))[l.segment + i] =
+        AdapterTile{l.adapter, l.begin + i * kAdapterSegment, min(l.rows - i * kAdapterSegment, kAdapterSegment),
+                    l.small + i * (kAdapterSegment / kAdapterSmallTile), l.large + i * (kAdapterSegment / kAdapterLargeTile),
+                    l.part < 0 ? -1 : l.part + i};
+}
+
+// One workgroup, for a plan serves every projection of a batch and is small beside them (150 rows 7.6 us, 8192 rows 22 us, 65536
+// rows 145 us; bound by the chain of two passes over the ids, 64 rows of a wave at a time).  Wave w takes the w-th stretch of
+// rows: it counts them by kind (adapter, or none = the last kind), a scan over kinds and waves gives every (kind, wave) its
+// place, and the wave puts its rows there in their order.
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) {
   extern __shared__ int count[];  // [waves][kinds]
   __shared__ int wave_sum[4][kPlanWaves];
@@ -120,22 +146,29 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int kind = tid * each + e;
-    if (e >= each || kind >= kinds) continue;
-    const int adapter = kind < a.adapters ? kind : -1, n = total[e], begin = before[0], small = before[1], large = before[2];
-    for (int i = 0; i < n; i += kAdapterSmallTile)
-      ((AdapterTile *)(a.plan + a.small))[before[1]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterSmallTile)};
-    for (int i = 0; i < n; i += kAdapterLargeTile)
-      ((AdapterTile *)(a.plan + a.large))[before[2]++] = AdapterTile{adapter, begin + i, min(n - i, kAdapterLargeTile)};
-    if (adapter >= 0) {
-      const int segments = (n + kAdapterSegment - 1) / kAdapterSegment;
+    const bool valid = e < each && kind < kinds;
+    Listed l = {valid && kind < a.adapters ? kind : -1, valid ? total[e] : 0, before[0], before[1], before[2], before[3], 0};
+    const int segments = l.adapter >= 0 ? (l.rows + kAdapterSegment - 1) / kAdapterSegment : 0;
+    l.part = segments > 1 ? part : -1;
+    // an adapter of few rows is listed by its thread, one of many by the wave
+    if (l.rows <= kAdapterLargeTile) list(a, l, 0, 1);
+    for (uint64_t many = __ballot(l.rows > kAdapterLargeTile); many; many &= many - 1) {
+      const int from = __builtin_ctzll(many);
+      const Listed other = {__builtin_amdgcn_readlane(l.adapter, from), __builtin_amdgcn_readlane(l.rows, from),
+                            __builtin_amdgcn_readlane(l.begin, from), __builtin_amdgcn_readlane(l.small, from),
+                            __builtin_amdgcn_readlane(l.large, from), __builtin_amdgcn_readlane(l.segment, from),
+                            __builtin_amdgcn_readlane(l.part, from)};
+      list(a, other, lane, 64);
+    }
+    if (!valid) continue;
+    if (l.adapter >= 0) {
       a.plan[a.parts + 2 * kind] = part, a.plan[a.parts + 2 * kind + 1] = segments;
-      for (int i = 0; i < n; i += kAdapterSegment)
-        ((AdapterTile *)(a.plan + a.segments))[before[3]++] =
-            AdapterTile{adapter, begin + i, min(n - i, kAdapterSegment), small + i / kAdapterSmallTile, large + i / kAdapterLargeTile,
-                        segments > 1 ? part + i / kAdapterSegment : -1};
       if (segments > 1) part += segments;
     }
-    int at = begin;
+    before[1] += (l.rows + kAdapterSmallTile - 1) / kAdapterSmallTile;
+    before[2] += (l.rows + kAdapterLargeTile - 1) / kAdapterLargeTile;
+    before[3] += segments;
+    int at = l.begin;
     for (int w = 0; w < kPlanWaves; ++w) {
       const int c = count[w * kinds + kind];
       count[w * kinds + kind] = at;
@@ -163,7 +196,8 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
 
 constexpr int kThreads = 256, kWaves = 4;
 
-// 8 values from p, of which `valid` exist (the rest are zeros); kWide: all or none of them, 16-byte aligned
+// 8 values from p, of which `valid` exist (the rest are zeros); kWide: all or none of them, 16-byte aligned.  Rows that are not
+// (4097 features to 4095, 4096 rows, rank 16) take 201 us where aligned ones of 4096 take 34, rank 15 with aligned rows 104.
 template <bool kWide>
 __device__ __forceinline__ half8_t load8(const half_t *p, int64_t valid) {
   half8_t v = {};

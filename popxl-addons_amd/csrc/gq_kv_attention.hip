@@ -17,6 +17,9 @@
 // takes units [U w / W, U (w + 1) / W), the four waves of it every fourth block.  A range may end inside a (sequence, head):
 // what it has then goes to the workspace and kv_join_kernel adds the parts, in the order of the blocks.  Nothing depends on
 // lengths that only the device knows, and results do not depend on timing.
+//
+// Measured: 64 sequences of up to 32768, 8 kv heads of 128, 4 query heads each: 376 us, 5.8 TB/s of codes; one sequence of 777, 16
+// heads of 256: 9 us, four dependent loads and the sums, and 4.6 us for kv_join_kernel.
 #include "gq_kv.h"
 
 namespace gq {
@@ -284,6 +287,12 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
 // Rescaling the accumulators for every block would cost as many vector instructions as the softmax.  The maximum in
 // use is only raised when scores pass it by more than 8 (probabilities up to 2^8 then), and the value scale enters the exponent
 // as its ratio to a reference, which only moves when the ratio leaves [1/16, 16]; the sum takes the ratio back out.
+//
+// Measured: 2 sequences of up to 2048 new tokens over 8000, 16 heads of 256: 450 to 500 us, 600 to 690 TFLOP/s (a large matrix
+// product: 1150).  Of a compute unit's time the matrix units are busy for 30 %, vector instructions for 33 %, and a third is waited:
+// with 330 registers a wave there is one to a SIMD, whose softmax nothing covers (products of the next scores moved among
+// it, by order or by scheduling barriers, took 520 to 590 us: the compiler then keeps fewer loads from LDS under way).
+// At 128 dims two waves share a SIMD: 4096 tokens, 32 heads: 195 us, 700 TFLOP/s.
 //
 // A grid too small for the device is divided over the keys as well: `splits` workgroups share a tile and kv_tile_join_kernel adds
 // their parts, in their order.

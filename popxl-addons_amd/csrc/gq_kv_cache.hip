@@ -11,8 +11,11 @@
 // scale is a maximum over all of it, and no other workgroup writes there.  The new tokens come by 16-byte loads that are
 // contiguous over a row and wait in LDS, as binary16, for the scale; from there key codes go out 8 dims at a time, and value
 // codes, which the cache holds transposed, 16 tokens of a dim at a time.  Keys that are turned on the way: the angles of the
-// block's tokens are formed once in LDS.  (With the tokens held in registers instead the kernel had 160
-// of them and 23 KiB of code, and a decode step waited for its instructions: 19 us for 48 requests.)
+// block's tokens are formed once in LDS.  (With the tokens held in registers instead the kernel had 160 of them and 23 KiB of
+// code, and a decode step waited for its instructions: 19 us for 48 requests.)  Measured, 8 heads of 128, keys turned, 16383
+// tokens: 25 us for the keys, 16 us for the values (2.5 and 4 TB/s; the angles and codes are what the keys wait for); a token
+// for each of 48 requests, 16 heads of 256: 11 us, most of it a chain of dependent loads (offsets, table, scale, tokens, the old
+// codes where the scale grows).
 #include "gq_kv.h"
 #include "gq_rotary.h"
 
@@ -21,7 +24,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kFewOfBlock = 4;  // new tokens of a sequence, on average, up to which a workgroup is one wave
-constexpr int kFew = 8;  // new tokens of a block up to which their value codes are stored byte by byte
+constexpr int kFew = 8;  // new tokens of a block up to which their value codes are stored byte by byte (with 2 in its place 2 ... 4
+                         // tokens of 48 sequences take 22 to 27 us, not 11 to 14; with 16 8 tokens of 8 sequences 10, not 11)
 
 struct AppendArgs {
   KvCache cache;
@@ -273,7 +277,9 @@ struct GatherArgs {
   half_t *out[2];
 };
 
-// The values of a batch's new tokens as binary16, [tokens][heads][dim]: one rounding of code * scale.
+// The values of a batch's new tokens as binary16, [tokens][heads][dim]: one rounding of code * scale.  A thread takes 4 tokens x 8
+// dims, so that values, which lie the other way round in the cache, are turned in registers.  Bound by memory: 1 byte read, 2
+// written an element; 16383 tokens, 8 heads of 128: 15.5 us, 6.5 TB/s (the codes are still in a cache behind the append).
 __global__ __launch_bounds__(kThreads) void kv_gather_kernel(GatherArgs a) {
   const int tid = threadIdx.x, h = blockIdx.x % a.cache.heads;
   const bool values = blockIdx.y != 0;
