@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void kv_split_kernel(At
 //
 // Measured: 2 sequences of up to 2048 new tokens over 8000, 16 heads of 256: 450 to 500 us, 600 to 690 TFLOP/s (a large matrix
 // product: 1150).  Of a compute unit's time the matrix units are busy for 30 %, vector instructions for 33 %, and a third is waited:
-// with 330 registers a wave there is one to a SIMD, whose softmax nothing covers (products of the next scores moved among
+// with 454 registers a wave there is one to a SIMD, whose softmax nothing covers (products of the next scores moved among
 // it, by order or by scheduling barriers, took 520 to 590 us: the compiler then keeps fewer loads from LDS under way).
 // At 128 dims two waves share a SIMD: 4096 tokens, 32 heads: 195 us, 700 TFLOP/s.
 //

@@ -24,8 +24,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kFewOfBlock = 4;  // new tokens of a sequence, on average, up to which a workgroup is one wave
-constexpr int kFew = 8;  // new tokens of a block up to which their value codes are stored byte by byte (with 2 in its place 2 ... 4
-                         // tokens of 48 sequences take 22 to 27 us, not 11 to 14; with 16 8 tokens of 8 sequences 10, not 11)
+// New tokens of a block up to which their value codes are stored byte by byte.  With 2 in its place up to 4 tokens of 48 sequences
+// take 22 to 27 us, not 11 to 14; with 8 up to 16 tokens of 48 sequences 27, not 25, up to 8 of 8 sequences 11, not 10.
+constexpr int kFew = 16;
 
 struct AppendArgs {
   KvCache cache;
