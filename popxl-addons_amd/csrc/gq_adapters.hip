@@ -893,6 +893,9 @@ int launch_up(const Batch &b, const float *v, int64_t splits, const half_t *w, c
   return GQ_BY_SHAPE(start_up, a, operands, stream);
 }
 
+// Workgroups at most for one adapter's weights, where every adapter gets as many and only the device knows which have rows.
+int64_t groups_of_adapter(int64_t adapters) { return adapters < 64 ? 512 : 32768 / adapters; }
+
 template <int kRank>
 int launch_outer(const OuterArgs &a, const PlanLayout &plan, bool wide, hipStream_t stream) {
   const int64_t features = a.side[0].features > a.side[1].features ? a.side[0].features : a.side[1].features;
@@ -903,8 +906,8 @@ int launch_outer(const OuterArgs &a, const PlanLayout &plan, bool wide, hipStrea
     adapter_outer_kernel<kRank, false><<<grid, kThreads, 0, stream>>>(a);
   const int rc = check_launch("adapter_outer_kernel");
   if (rc != GQ_OK) return rc;
-  const int64_t each = (a.rank * features + kThreads - 1) / kThreads;
-  adapter_sum_kernel<<<dim3((unsigned)(each < 1024 ? each : 1024), (unsigned)a.adapters, 2), kThreads, 0, stream>>>(a);
+  const int64_t each = (a.rank * features + kThreads - 1) / kThreads, most = 2 * groups_of_adapter(a.adapters);
+  adapter_sum_kernel<<<dim3((unsigned)(each < most ? each : most), (unsigned)a.adapters, 2), kThreads, 0, stream>>>(a);
   return check_launch("adapter_sum_kernel");
 }
 
@@ -975,8 +978,9 @@ int launch_adapter_grad(const gq_adapters &w, const void *plan, int64_t rows, co
   char *ws = (char *)workspace;
   half_t *down_turned = (half_t *)(ws + l.turned[0]), *up_turned = (half_t *)(ws + l.turned[1]);
   const int64_t pieces = ((in > out ? in : out) + 63) / 64 * ((w.rank + 63) / 64);
+  const int64_t most_pieces = groups_of_adapter(w.n_adapters);
   const TurnArgs turn = {{(const half_t *)w.down, (const half_t *)w.up}, {down_turned, up_turned}, {w.rank, out}, {in, w.rank},
-                         b.words + b.plan.parts, (int)(pieces < 512 ? pieces : 512), (int)w.n_adapters,
+                         b.words + b.plan.parts, (int)(pieces < most_pieces ? pieces : most_pieces), (int)w.n_adapters,
                          (w.rank | in | out) % 8 == 0 && aligned16(w.down) && aligned16(w.up)};
   int rc = launch_down(b, (const half_t *)x, x_stride, (const half_t *)w.down, in, w.rank, (float *)(ws + l.v), (float *)(ws + l.most[0]), in_splits,
                        &turn, stream);
