@@ -17,7 +17,7 @@
 //
 // Measured (TB/s of rows): 6001 rows, 4096 to 12288, rank 32: adapter_down_kernel 23 us (2.1), adapter_up_kernel 73 us (4.0).
 // Gradients of 8192 rows, 4096 to 16384, rank 64: x A^T 28 us (2.4, the turned weights with it), dy B 77 us (3.5), dx 42 us
-// (3.2, the operands with it), the outer products 105 us (3.2), their sum 9 us.  A decode batch of 8 rows: 4 and 4.4 us, two launches.
+// (3.2, the operands with it), the outer products 101 us (3.3), their sum 9 us.  A decode batch of 8 rows: 4 and 4.4 us, two launches.
 #include "gq_adapters.h"
 
 namespace gq {
