@@ -527,8 +527,9 @@ struct UpArgs {
 
 // The workgroup sums its rows' v over the splits into LDS, where its waves take their operands from.  Then wave w takes 64
 // features at a time: row 4 g' + i of operand tile f is feature 32 (f / 2) + 8 g' + 4 (f % 2) + i, so that a lane ends with 8
-// consecutive features of one row in each half (16-byte loads and stores, 64 bytes of a row together).  The weights and y of the next
-// piece are loaded before and among this one's products.
+// consecutive features of one row in each half.  From there they go through the wave's own LDS to the lanes that have these rows
+// of y, 8 to a row: loads and stores are whole lines (stored by halves of a line from the accumulators' own lanes, 6001 rows to 12288
+// took 88 us, so 73).  The weights and y of the next piece are loaded before and among this one's products.
 template <int kRank, int kTiles, bool kWide>
 __global__ __launch_bounds__(kThreads, kRank * kTiles > 256 ? 1 : 2) void adapter_up_kernel(UpArgs a) {
   constexpr int kChunks = kRank / 32, kRow = kRank + 4, kTurned = 64 + 4;
