@@ -1,7 +1,17 @@
-"""Small host-side containers used by the layers: named variables and a validating weight map."""
+"""Small host-side helpers: the layers' named variables and validating weight map, modules that are called as their function."""
+import sys
+import types
 from collections.abc import MutableMapping
 
 import numpy as np
+
+
+def callable_module(name, function):
+    """Let the module `name` be called as `function`, which it holds under its own last name: whoever imports that name from
+    the package above gets both, whichever was imported first."""
+    module = sys.modules[name]
+    module.__class__ = type("CallableModule", (types.ModuleType,), {"__call__": staticmethod(function)})
+    module.__wrapped__ = function  # (its signature)
 
 
 class Variable:
