@@ -15,20 +15,13 @@ BLOCK = 64  # tokens of one block of the cache, the unit that has a scale of its
 BASE = 10000.0
 
 
-_ops = None
-
-
 def _framework():
-    """popxl_addons.ops, imported at the first call (a program imports it once, not with every call of an operator)."""
-    global _ops
-    if _ops is None:
-        path = os.path.join(os.getcwd(), "popxl-addons_amd")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        from popxl_addons import ops
+    path = os.path.join(os.getcwd(), "popxl-addons_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from popxl_addons.ops import kv_cache_gq, low_rank_adapters, rotary_pos_embed
 
-        _ops = ops
-    return _ops
+    return rotary_pos_embed, kv_cache_gq, low_rank_adapters
 
 
 # ------------------------------------------------------------------------------------------------- cases
@@ -189,7 +182,8 @@ def prepare(case, seed):
                  positions=torch.randint(0, case["positions"], (t,), generator=gen, device="cuda", dtype=torch.int32),
                  w=w.cuda(), factor=factor)
         if own:
-            s["rotary"] = _framework().RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"], scaling=_SCALING[case["scaling"]])
+            rotary = _framework()[0]
+            s["rotary"] = rotary.RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"], scaling=_SCALING[case["scaling"]])
     elif op in ("append", "attend"):
         _paged(case, gen, order, s)
         t, h, d = sum(s["fresh"]), case["kv_heads"], case["head_dim"]
@@ -203,10 +197,10 @@ def prepare(case, seed):
         else:
             s["q"] = _normal(gen, t, case["q_heads"], d)
         if own:
-            ops = _framework()
-            s["cache"] = ops.KVCacheGQ.from_tensors(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"])
+            rotary, kv_cache, _ = _framework()
+            s["cache"] = kv_cache.KVCacheGQ.from_tensors(s["k_codes"], s["v_codes"], s["k_scale"], s["v_scale"])
             if op == "append":
-                s["rotary"] = ops.RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"])
+                s["rotary"] = rotary.RotaryPosEmbed(case["rotary_dim"], base=BASE, layout=case["layout"])
     else:
         m, k, n, r, na = (case[x] for x in ("rows", "k", "n", "rank", "adapters"))
         kinds = na + (1 if case["none"] else 0)
@@ -222,9 +216,9 @@ def prepare(case, seed):
         else:
             s["dy"], s["dx"] = _normal(gen, m, n, std=1e-2), _normal(gen, m, k, std=1e-2)
         if own:
-            ops = _framework()
-            s["adapters"] = ops.LowRankAdapters(s["down"], s["up"], s["scaling"])
-            s["plan"] = ops.AdapterPlan(s["ids"], na)
+            lora = _framework()[2]
+            s["adapters"] = lora.LowRankAdapters(s["down"], s["up"], s["scaling"])
+            s["plan"] = lora.AdapterPlan(s["ids"], na)
     return s
 
 
@@ -326,18 +320,18 @@ def _plain_adapt_back(s):
 def run(state):
     s, op = state, state["case"]["op"]
     if own:
-        ops = _framework()
+        rotary, kv_cache, lora = _framework()
         if op == "rotary":
-            return ops.rotary_pos_embed(s["t"], s["positions"], s["rotary"], inverse=s["case"]["inverse"])
+            return rotary.rotary_pos_embed(s["t"], s["positions"], s["rotary"], inverse=s["case"]["inverse"])
         if op == "append":
-            ops.kv_cache_append(s["cache"], s["k"], s["v"], s["offsets"], s["seq_lens"], s["table"], rotary=s["rotary"])
-            k, v = ops.kv_cache_gather(s["cache"], s["offsets"], s["seq_lens"], s["table"], tokens=s["k"].shape[0])
+            kv_cache.kv_cache_append(s["cache"], s["k"], s["v"], s["offsets"], s["seq_lens"], s["table"], rotary=s["rotary"])
+            k, v = kv_cache.kv_cache_gather(s["cache"], s["offsets"], s["seq_lens"], s["table"], tokens=s["k"].shape[0])
             return {"k": k, "v": v}
         if op == "attend":
-            return ops.kv_cache_attention(s["q"], s["cache"], s["offsets"], s["seq_lens"], s["table"])
+            return kv_cache.kv_cache_attention(s["q"], s["cache"], s["offsets"], s["seq_lens"], s["table"])
         if op == "adapt":
-            return ops.low_rank_adapters(s["x"], s["y"], s["adapters"], s["plan"], activation=s["case"]["activation"] or None)
-        dx, d_down, d_up = ops.low_rank_adapters_grad(s["x"], s["dy"], s["adapters"], s["plan"], dx=s["dx"])
+            return lora.low_rank_adapters(s["x"], s["y"], s["adapters"], s["plan"], activation=s["case"]["activation"] or None)
+        dx, d_down, d_up = lora.low_rank_adapters_grad(s["x"], s["dy"], s["adapters"], s["plan"], dx=s["dx"])
         return {"dx": dx, "d_down": d_down, "d_up": d_up}
     if op == "rotary":
         return _rotated(s["t"], s["positions"], s["w"], s["factor"], s["case"]["layout"], s["case"]["inverse"])
