@@ -170,7 +170,7 @@ def low_rank_adapters_grad(x, dy, adapters, plan, dx=None):
     out = x.new_empty(x.shape)
     if plan.rows == 0 or adapters.in_features == 0 or adapters.out_features == 0:
         d_down, d_up = (torch.zeros(w.shape, dtype=torch.float32, device=w.device) for w in (adapters.down, adapters.up))
-        return out if dx is None else out.copy_(dx), d_down, d_up
+        return out.zero_() if dx is None else out.copy_(dx), d_down, d_up
     d_down, d_up = (torch.empty(w.shape, dtype=torch.float32, device=w.device) for w in (adapters.down, adapters.up))
     workspace, nbytes = adapters.workspace("gq_adapter_grad_workspace_bytes", plan.rows)
     _gq_hip.launch(adapters.index, "gq_adapter_grad_f16", ctypes.byref(adapters._c), plan.data.data_ptr(), plan.rows, x2.data_ptr(),

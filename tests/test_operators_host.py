@@ -2,6 +2,7 @@
 frequencies of stretched contexts."""
 import ctypes
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -253,3 +254,23 @@ def test_python_calls_refuse_cpu_tensors_types_and_shapes():
         layer.grad(x)
     with pytest.raises(ValueError):
         low_rank_adapters(x, x, adapters, plan=type("Plan", (), dict(n_adapters=3, device=adapters.device, rows=3))())
+
+
+@pytest.mark.parametrize("rows,k,n", [(3, 64, 0), (0, 64, 32), (3, 0, 32)])
+@pytest.mark.parametrize("with_dx", [False, True])
+def test_gradients_without_rows_or_features(monkeypatch, rows, k, n, with_dx):
+    """No dx stands for zeros, also where there is nothing to add to them.  (These sizes launch nothing: CPU tensors do, once the
+    check for GPU ones is taken away; new memory is filled with NaN.)"""
+    module = sys.modules["popxl_addons.ops.low_rank_adapters.low_rank_adapters"]
+    monkeypatch.setattr(module, "_matrix", lambda name, t, *rest: t)
+    adapters = LowRankAdapters(torch.ones((2, 4, k), dtype=torch.float16), torch.ones((2, n, 4), dtype=torch.float16))
+    plan = type("Plan", (), dict(n_adapters=2, device=adapters.device, index=adapters.index, rows=rows))()
+    x, dy = torch.ones((rows, k), dtype=torch.float16), torch.ones((rows, n), dtype=torch.float16)
+    dx = torch.full((rows, k), 2.0, dtype=torch.float16) if with_dx else None
+    torch.use_deterministic_algorithms(True)
+    try:
+        got, d_down, d_up = module.low_rank_adapters_grad(x, dy, adapters, plan, dx=dx)
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert torch.equal(got, torch.zeros_like(x) if dx is None else dx) and got is not dx
+    assert d_down.dtype == d_up.dtype == torch.float32 and not d_down.any() and not d_up.any()
