@@ -829,13 +829,6 @@ struct Batch {
   int64_t most_tiles() const { return large ? plan.most_large : plan.most_small; }
 };
 
-// A kernel has to be told of more than 64 KiB of LDS, on each device.
-int allow_lds(const void *kernel, size_t bytes, const char *who) {
-  if (bytes <= 64 << 10) return GQ_OK;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? GQ_OK : fail((int)e, "%s: %s", who, hipGetErrorString(e));
-}
-
 template <int kRank, int kTiles, bool kWide>
 int start_down(const DownArgs &a, int64_t turns, hipStream_t stream) {
   const size_t sums = (size_t)kWaves * 16 * (kRank + 4) * sizeof(float), turned = turns ? 64 * 72 * sizeof(half_t) : 0;
@@ -944,7 +937,8 @@ int launch_adapter_plan(const int32_t *ids, int64_t rows, int64_t adapters, void
   const PlanLayout l(rows, adapters);
   const PlanArgs a = {ids, (int *)plan, l.counts, l.order, l.parts, l.small, l.large, l.segments, (int)rows, (int)adapters};
   const size_t lds = (size_t)kPlanWaves * (adapters + 1) * sizeof(int);
-  if (int rc = allow_lds((const void *)adapter_plan_kernel, lds, "adapter_plan_kernel")) return rc;
+  constexpr size_t most = (size_t)kPlanWaves * (kMostAdapters + 1) * sizeof(int);
+  if (const int rc = allow_lds<adapter_plan_kernel, most>(lds, "adapter_plan_kernel")) return rc;
   adapter_plan_kernel<<<1, kPlanThreads, lds, stream>>>(a);
   return check_launch("adapter_plan_kernel");
 }

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gq_hip.h"
 
 namespace gq {
@@ -11,6 +13,24 @@ namespace gq {
 int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 // Maps the runtime's last launch error (if any) to a return code, recording its text.
 int check_launch(const char *what);
+
+// A kernel that may use more LDS than any launch gets (64 KiB with its static arrays) has to be allowed to, on each device.  The
+// limit is the kernel's, shared by all threads, so it is set to the most that any call of the kernel uses, once: a call that set
+// what it needs itself would lower it under another thread's launch.  `lds`: what this launch uses.
+template <auto kKernel, size_t kMost>
+int allow_lds(size_t lds, const char *who) {
+  static_assert(kMost <= 160 << 10, "LDS of a compute unit");
+  if (lds <= 60 << 10) return GQ_OK;
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> allowed[kMaxDevices];  // (two threads may both set it: to the same value)
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) return fail(GQ_ERR_NO_DEVICE, "%s: no current device", who);
+  if (allowed[dev]) return GQ_OK;
+  const hipError_t e = hipFuncSetAttribute((const void *)kKernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
+  if (e != hipSuccess) return fail((int)e, "%s: %s", who, hipGetErrorString(e));
+  allowed[dev] = true;
+  return GQ_OK;
+}
 
 // A block of device memory that the library keeps per GPU and every call on that GPU shares (the
 // progress words of gq_gemv_sequence_f16, the scratch of gq_linear_kn_act_noalloc_f16): calls

@@ -633,17 +633,10 @@ __global__ __launch_bounds__(kThreads) void kv_join_kernel(AttentionArgs a) {
   }
 }
 
-// A kernel has to be told of more than 64 KiB of LDS, on each device.
-int allow_lds(const void *kernel, size_t bytes, const char *who) {
-  if (bytes <= 64 << 10) return GQ_OK;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? GQ_OK : fail((int)e, "%s: %s", who, hipGetErrorString(e));
-}
-
 template <int DP>
 int launch_split(const AttentionArgs &a, hipStream_t stream) {
-  const size_t lds = (size_t)kWaves * kRows * (DP + 4 + 2) * sizeof(float);
-  if (const int rc = allow_lds((const void *)kv_split_kernel<DP>, lds, "kv_split_kernel")) return rc;
+  constexpr size_t lds = (size_t)kWaves * kRows * (DP + 4 + 2) * sizeof(float);
+  if (const int rc = allow_lds<kv_split_kernel<DP>, lds>(lds, "kv_split_kernel")) return rc;
   kv_split_kernel<DP><<<a.groups, kThreads, lds, stream>>>(a);
   return check_launch("kv_split_kernel");
 }
@@ -663,8 +656,8 @@ int tile_splits(int64_t groups, int64_t dim, int64_t width) {
 
 template <int DP>
 int launch_tile(AttentionArgs &a, hipStream_t stream) {
-  const size_t lds = (size_t)2 * 2 * kBlock * DP * sizeof(half_t);
-  if (const int rc = allow_lds((const void *)kv_tile_kernel<DP>, lds, "kv_tile_kernel")) return rc;
+  constexpr size_t lds = (size_t)2 * 2 * kBlock * DP * sizeof(half_t);
+  if (const int rc = allow_lds<kv_tile_kernel<DP>, lds>(lds, "kv_tile_kernel")) return rc;
   const int64_t groups = tile_groups(a.batch, a.cache.heads, a.group);
   if (groups > 0x7fffff) return fail(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16: too many rows for one launch");
   a.groups = (int)groups, a.splits = tile_splits(groups, a.cache.dim, a.batch.width);

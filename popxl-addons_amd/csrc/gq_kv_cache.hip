@@ -325,12 +325,8 @@ __global__ __launch_bounds__(kThreads) void kv_gather_kernel(GatherArgs a) {
   }
 }
 
-// A kernel has to be told of more than 64 KiB of LDS, on each device.
-int allow_lds(const void *kernel, size_t bytes) {
-  if (bytes <= 63 << 10) return GQ_OK;
-  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? GQ_OK : fail((int)e, "kv_append_kernel: %s", hipGetErrorString(e));
-}
+// A block's tokens of 256 dims and the angles of 128 pairs.
+constexpr size_t kMostLds = kBlock * (256 * sizeof(half_t) + 128 * sizeof(float2));
 
 // (sequence, block) pairs at most: a sequence of n new tokens reaches into (n + 62) / 64 + 1 blocks
 int64_t most_places(const KvBatch &b) { return b.tokens / kBlock + 2 * (int64_t)b.sequences; }
@@ -357,13 +353,13 @@ int launch_kv_append(const KvCache &cache, const KvBatch &batch, const uint16_t 
   // Blocks of few tokens: one wave each (48 sequences of 1, about 2, about 4 tokens, 16 heads of 256: 11, 15, 27 us, with four waves
   // 14, 17, 21; 8 sequences of 1, about 8 tokens, 8 heads of 128: 5.5 and 11, with four waves 10 and 12).
   if (batch.tokens < kFewOfBlock * batch.sequences) {
-    if (const int rc = allow_lds((const void *)kv_append_kernel<64>, codes + angles)) return rc;
+    if (const int rc = allow_lds<kv_append_kernel<64>, kMostLds>(codes + angles, "kv_append_kernel")) return rc;
     kv_append_kernel<64><<<dim3((unsigned)(places * cache.heads), 2), 64, codes + angles, stream>>>(a);
   } else {
     // Keys and values apart: the angles take as much LDS as the rows or twice that, which only the keys' workgroups need.
     // (Sharing the angles between four heads of a workgroup took 47 us where this takes 43, for 16383 tokens, 8 heads of 128, and
     // 45 where this takes 28, for 48 sequences of about 8 tokens, 16 heads of 256.)
-    if (const int rc = allow_lds((const void *)kv_append_kernel<kThreads>, codes + angles)) return rc;
+    if (const int rc = allow_lds<kv_append_kernel<kThreads>, kMostLds>(codes + angles, "kv_append_kernel")) return rc;
     kv_append_kernel<kThreads><<<(unsigned)(places * cache.heads), kThreads, codes + angles, stream>>>(a);
     a.first = 1;
     kv_append_kernel<kThreads><<<(unsigned)(places * cache.heads), kThreads, codes, stream>>>(a);
