@@ -171,6 +171,7 @@ def load():
         fn = getattr(lib, name)
         fn.argtypes = [p, p, p, p, p, i64, i64, i64, p]
         fn.restype = ctypes.c_int
+    lib.hipStreamGetCaptureInfo.restype, lib.hipStreamGetCaptureInfo.argtypes = ctypes.c_int, [p, p, p]  # (the runtime's, which the library is linked to)
     i32, f32 = ctypes.c_int32, ctypes.c_float
     for name, result, arguments in (
         ("gq_rotary_f16", ctypes.c_int, [p, i64, i64, p, p, i32, p, i64, i64, i64, i64, i64, p]),
@@ -216,27 +217,49 @@ def launch(index, name, *args):
         return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-_kn_workspaces = {}
+def _capture_of(stream):
+    """The number of the graph capture that `stream` (a raw handle) is in; None if it is in none."""
+    if not stream:  # (the default stream cannot be captured)
+        return None
+    status, number = ctypes.c_int(0), ctypes.c_ulonglong(0)
+    rc = load().hipStreamGetCaptureInfo(stream, ctypes.byref(status), ctypes.byref(number))
+    if rc != 0:
+        raise GQHipError("hipStreamGetCaptureInfo", rc, f"is stream {stream:#x} a stream?")
+    return None if status.value == 0 else number.value
+
+
+_kn_workspaces = {}        # (device, stream): the buffer of eager calls
+_captured_workspaces = {}  # (device, stream): the last capture there and its buffer
 
 
 def linear_kn_workspace(device, nbytes):
     """The scratch buffer of gq_linear_kn_act_f16 and gq_linear_act_ws_f16 for calls enqueued on the
     CURRENT stream of `device`: one buffer per (device, stream), grown on demand; its arrival counters
     start at zero and every call leaves them zero.  Calls that share a buffer are on the same stream
-    and therefore ordered; layers built on different streams get different buffers and may overlap."""
+    and therefore ordered; layers built on different streams get different buffers and may overlap.
+    A stream under capture gets a buffer of that capture: its zeroing is part of the graph, which may be
+    replayed first, beside other graphs and eager calls, or after any of them asked for a larger one."""
     import torch
 
     device = torch.device(device)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
     key = (device, torch.cuda.current_stream(device).cuda_stream)
-    ws = _kn_workspaces.get(key)
+    capture = _capture_of(key[1])
+    if capture is None:
+        ws = _kn_workspaces.get(key)
+    else:
+        number, ws = _captured_workspaces.get(key, (None, None))
+        ws = ws if number == capture else None
     if ws is None or ws.numel() < nbytes:
         with torch.cuda.device(device):
-            # (a buffer that is being replaced stays alive until the work enqueued on it has run:
-            # the caching allocator hands its memory out again on the same stream only)
+            # (a buffer that is being replaced stays alive until the work enqueued on it has run: the caching
+            # allocator hands its memory out again on the same stream, a captured one's to the same graph, only)
             ws = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-        _kn_workspaces[key] = ws
+        if capture is None:
+            _kn_workspaces[key] = ws
+        else:
+            _captured_workspaces[key] = capture, ws
     return ws
 
 

@@ -301,3 +301,43 @@ def test_weights_dict_validates_dtype_and_shape():
     assert nt.w is var and nt["w"] is var and "w" in nt
     with pytest.raises(AttributeError):
         nt.missing
+
+
+def test_workspaces_of_captured_calls_are_their_capture_s(monkeypatch):
+    """A buffer of the arrival counters belongs to one stream's eager calls or to one stream of one capture: what a graph uses is
+    zeroed by that graph, and no other graph or eager call writes there."""
+    import contextlib
+    import types
+
+    now = types.SimpleNamespace(stream=7, capture=None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=now.stream))
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(_gq_hip, "_capture_of", lambda stream: now.capture, raising=False)
+    monkeypatch.setattr(_gq_hip, "_kn_workspaces", {})
+    monkeypatch.setattr(_gq_hip, "_captured_workspaces", {}, raising=False)
+    held = []
+
+    def workspace(stream, capture, nbytes):
+        now.stream, now.capture = stream, capture
+        ws = _gq_hip.linear_kn_workspace("cpu:0", nbytes)
+        assert ws.numel() >= nbytes
+        held.append(ws)
+        return ws
+
+    eager = workspace(7, None, 100)
+    eager.fill_(1)  # (what calls leave is zeros; here it tells the buffers apart)
+    first = workspace(7, 1, 100)
+    assert first is not eager and not first.any()
+    first.fill_(2)
+    assert workspace(7, 1, 50) is first  # ordered by the stream, zeroed once
+    assert workspace(8, 1, 50) is not first  # another stream of the capture
+    larger = workspace(7, 1, 3 << 20)
+    assert larger is not first and not larger.any() and workspace(7, 1, 100) is larger
+    second = workspace(7, 2, 100)
+    assert second is not larger and second is not first and not second.any()
+    assert workspace(7, None, 100) is eager and workspace(7, 3, 100) is not second
+    assert len({ws.data_ptr() for ws in (eager, first, larger, second)}) == 4
+
+
+def test_default_stream_is_in_no_capture():
+    assert _gq_hip._capture_of(0) is None
