@@ -113,12 +113,18 @@ int launch_rotary(const uint16_t *t, int64_t t_token, int64_t t_head, const int3
   const int64_t most = (heads + least - 1) / least;
   groups = groups < most ? groups : most;
   a.heads_per_group = (int)((heads + groups - 1) / groups);
-  const dim3 grid((unsigned)tokens, (unsigned)((heads + a.heads_per_group - 1) / a.heads_per_group));
-  if (vec)
-    rotary_kernel<true><<<grid, kThreads, 0, stream>>>(a);
-  else
-    rotary_kernel<false><<<grid, kThreads, 0, stream>>>(a);
-  return check_launch("rotary_kernel");
+  const unsigned across = (unsigned)((heads + a.heads_per_group - 1) / a.heads_per_group);
+  constexpr int64_t kMostTokens = 1 << 23;  // of a launch: a grid has fewer than 2^32 threads along an axis
+  for (int64_t first = 0; first < tokens; first += kMostTokens) {
+    const dim3 grid((unsigned)(tokens - first < kMostTokens ? tokens - first : kMostTokens), across);
+    if (vec)
+      rotary_kernel<true><<<grid, kThreads, 0, stream>>>(a);
+    else
+      rotary_kernel<false><<<grid, kThreads, 0, stream>>>(a);
+    if (const int rc = check_launch("rotary_kernel")) return rc;
+    a.t += kMostTokens * t_token, a.out += kMostTokens * o_token, a.positions += kMostTokens;
+  }
+  return GQ_OK;
 }
 
 }  // namespace gq

@@ -112,3 +112,17 @@ def test_empty_and_other_stream(hip, device):
         got = rotary_pos_embed(t, positions, rotary)
     stream.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dim,tokens", [(16, 1 << 24), (2, (1 << 24) - 3)])
+def test_most_tokens(hip, device, dim, tokens):
+    """As many tokens as a call takes are more than a grid holds: the bits of calls on parts of them."""
+    gen = torch.Generator(device=device).manual_seed(dim)
+    t = torch.randn((tokens, 1, dim), generator=gen, device=device, dtype=torch.float16)
+    positions = torch.randint(-2 ** 31, 2 ** 31 - 1, (tokens,), generator=gen, device=device, dtype=torch.int32)
+    rotary = RotaryPosEmbed(dim, device=device)
+    got, third = rotary_pos_embed(t, positions, rotary), tokens // 3
+    for i in range(0, tokens, third):
+        assert torch.equal(got[i:i + third], rotary_pos_embed(t[i:i + third], positions[i:i + third], rotary)), i
+    assert rotary_pos_embed(t, positions, rotary, out=t) is t
+    assert torch.equal(got, t)

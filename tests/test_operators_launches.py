@@ -47,3 +47,50 @@ def test_limits_of_lds_are_the_same_for_every_call():
     for key, values in limits.items():
         assert len(values) == 1, (key, values)
         assert most[key] <= values[0] <= 160 << 10
+
+
+def rotary(tokens, heads, dim, rotary_dim, device=0):
+    return [device, "gq_rotary_f16", [FAKE, heads * dim, dim, FAKE, ["Rotary", FAKE, 1.0, rotary_dim, 0], 0, 2 * FAKE, heads * dim, dim, tokens, heads, dim, None]]
+
+
+def gather(tokens, sequences, heads, dim, device=0):
+    cache = ["KvCache", FAKE, FAKE, FAKE, FAKE, 10, heads, dim]
+    return [device, "gq_kv_gather_f16", [cache, ["KvBatch", FAKE, FAKE, FAKE, sequences, 4, tokens], FAKE, 2 * FAKE, None]]
+
+
+def adapters(rows, count, rank, k, n, grad, device=0):
+    w = ["Adapters", FAKE, FAKE, FAKE, count, rank, k, n]
+    if grad:
+        return [device, "gq_adapter_grad_f16", [w, FAKE, rows, FAKE, k, 3 * FAKE, n, None, 0, 2 * FAKE, k, FAKE, FAKE, FAKE, 1 << 62, None]]
+    return [device, "gq_adapter_apply_f16", [w, FAKE, rows, FAKE, k, 3 * FAKE, n, 2 * FAKE, n, 0, FAKE, 1 << 62, None]]
+
+
+MOST = 1 << 24  # tokens, rows
+UNSUPPORTED = -4
+LARGEST = [
+    rotary(MOST, 1, 16, 16), rotary(MOST - 1, 65535, 64, 32), rotary(MOST, 40, 128, 128), rotary((1 << 23) + 1, 3, 33, 2), rotary(1, 65535, 2048, 256),
+    append(MOST, 1, 1, 128, 128), append(MOST, 1, 8, 128), append(MOST, 1 << 20, 1, 16), append(1 << 20, 1 << 20, 1, 64), gather(MOST, 1, 8, 128),
+    attend(MOST, 1, 1, 128, 1), attend(1 << 20, 1 << 20, 1, 64, 8), attend(1 << 14, 1, 1024, 16, 65536 - 1024, 1 << 24), attend(1 << 14, 1 << 14, 8, 256, 32, 1 << 20),
+    plan(MOST, 2048), plan(MOST, 1),
+    *(adapters(rows, count, rank, k, n, grad) for grad in (False, True)
+      for rows, count, rank, k, n in ((MOST, 2048, 128, 4096, 4096), (MOST, 1, 8, 4097, 33), (8191, 2048, 16, 1 << 20, 1 << 20), (1, 2048, 1, 1 << 20, 1))),
+]
+
+
+def test_largest_sizes_fit_a_grid():
+    """Whatever is not refused is launched as grids that exist: fewer than 2^32 threads an axis, 65535 workgroups along y and z."""
+    for call, result in zip(LARGEST, launches(LARGEST)):
+        assert result["code"] in (0, UNSUPPORTED), (call, result["code"])
+        assert bool(result["records"]) == (result["code"] == 0), call
+        for r in result["records"]:
+            if r["launch"]:
+                assert all(0 < g and g * b < 1 << 32 for g, b in zip(r["grid"], r["block"])), (call, r)
+                assert r["grid"][1] <= 65535 and r["grid"][2] <= 65535, (call, r)
+
+
+def test_rotary_takes_as_many_tokens_as_it_says():
+    calls = [rotary(tokens, 3, 64, 32) for tokens in (1, 511, MOST // 2, MOST // 2 + 1, MOST - 1, MOST)]
+    for call, result in zip(calls, launches(calls)):
+        assert result["code"] == 0
+        assert sum(r["grid"][0] for r in result["records"]) == call[2][9]
+    assert launches([rotary(MOST + 1, 1, 64, 32)])[0]["code"] == UNSUPPORTED
