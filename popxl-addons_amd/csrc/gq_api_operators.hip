@@ -162,6 +162,8 @@ int gq_kv_attention_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, cons
   if (gq::misaligned(q, 16) || (q_token_stride | q_head_stride) % 8 != 0 || gq::misaligned(out, 2))
     return gq::fail(GQ_ERR_MISALIGNED, "%s: every row of q must be 16-byte aligned (strides multiples of 8), out 2-byte", who);
   if (const int bad = gq::check_workspace(who, workspace, workspace_bytes, gq::kv_attention_workspace_bytes(cache->head_dim), 16)) return bad;
+  if (out == q)  // (a row of q is read by the workgroups of several ranges of blocks)
+    return gq::fail(GQ_ERR_UNSUPPORTED, "%s: out must not be q", who);
   return gq::launch_kv_attention(c, b, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, q_heads, scale,
                                  workspace, (hipStream_t)stream);
 }

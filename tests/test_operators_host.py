@@ -274,3 +274,12 @@ def test_gradients_without_rows_or_features(monkeypatch, rows, k, n, with_dx):
         torch.use_deterministic_algorithms(False)
     assert torch.equal(got, torch.zeros_like(x) if dx is None else dx) and got is not dx
     assert d_down.dtype == d_up.dtype == torch.float32 and not d_down.any() and not d_up.any()
+
+
+def test_attention_apart_from_its_queries():
+    """Several workgroups read a row of q when others have written the result there."""
+    cache, batch = _gq_hip.KvCache(16, 16, 16, 16, 10, 2, 64), _gq_hip.KvBatch(16, 16, 16, 3, 4, 5)
+    for token_stride, head_stride in ((256, 64), (64, 320)):  # (the same start is the same first row, whatever the strides)
+        message = _refused(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16", _address(cache), _address(batch), 16, 256, 64, 16, token_stride, head_stride,
+                           4, 1.0, 16, 1 << 40, None)
+        assert "out must not be q" in message
