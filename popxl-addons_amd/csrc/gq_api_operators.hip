@@ -50,6 +50,13 @@ int check_kv(const char *who, const gq_kv_cache *cache, const gq_kv_batch *batch
 
 bool bad_stride(int64_t s) { return s < 0 || s > kLargest; }
 
+// a result that is one place of memory many times; the kernels write its rows in no order
+int check_apart(const char *who, int64_t rows, int64_t stride, int64_t least) {
+  return rows > 1 && stride < least ? fail(GQ_ERR_UNSUPPORTED, "%s: rows of the result lie on each other (%lld of them %lld elements apart)", who,
+                                           (long long)rows, (long long)stride)
+                                    : GQ_OK;
+}
+
 // 1: proceed; 0: nothing to do; negative: refused
 int check_adapters(const char *who, const gq_adapters *w, int64_t rows) {
   if (!w) return fail(GQ_ERR_NULL_POINTER, "%s: adapters is NULL", who);
@@ -101,6 +108,8 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: a stride is negative or exceeds 2^30", who);
   if (t == out && (t_token_stride != out_token_stride || t_head_stride != out_head_stride))
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: in place, t and out must have the same strides", who);
+  if (const int rc = gq::check_apart(who, tokens, out_token_stride, 1)) return rc;
+  if (const int rc = gq::check_apart(who, heads, out_head_stride, 1)) return rc;
   return gq::launch_rotary(t, t_token_stride, t_head_stride, positions, *rotary, inverse != 0, out, out_token_stride,
                            out_head_stride, tokens, heads, head_dim, (hipStream_t)stream);
 }
@@ -135,6 +144,7 @@ int gq_kv_gather_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, uint16_
   if (rc <= 0) return rc;
   if (!k || !v) return gq::fail(GQ_ERR_NULL_POINTER, "%s: k and v must not be NULL", who);
   if (gq::misaligned(k, 16) || gq::misaligned(v, 16)) return gq::fail(GQ_ERR_MISALIGNED, "%s: k and v must be 16-byte aligned", who);
+  if (k == v) return gq::fail(GQ_ERR_UNSUPPORTED, "%s: the results lie on each other", who);
   return gq::launch_kv_gather(c, b, k, v, (hipStream_t)stream);
 }
 
@@ -164,6 +174,8 @@ int gq_kv_attention_f16(const gq_kv_cache *cache, const gq_kv_batch *batch, cons
   if (const int bad = gq::check_workspace(who, workspace, workspace_bytes, gq::kv_attention_workspace_bytes(cache->head_dim), 16)) return bad;
   if (out == q)  // (a row of q is read by the workgroups of several ranges of blocks)
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: out must not be q", who);
+  if (const int bad = gq::check_apart(who, b.tokens, out_token_stride, 1)) return bad;
+  if (const int bad = gq::check_apart(who, q_heads, out_head_stride, 1)) return bad;
   return gq::launch_kv_attention(c, b, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, q_heads, scale,
                                  workspace, (hipStream_t)stream);
 }
@@ -212,6 +224,8 @@ int gq_adapter_apply_f16(const gq_adapters *adapters, const void *plan, int64_t 
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: a stride is negative or exceeds 2^30", who);
   if (y == out && y_row_stride != out_row_stride)
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: in place, y and out must have the same stride", who);
+  rc = gq::check_apart(who, rows, out_row_stride, adapters->out_features);
+  if (rc != GQ_OK) return rc;
   rc = gq::check_workspace(who, workspace, workspace_bytes,
                            gq::adapter_apply_workspace_bytes(rows, adapters->n_adapters, adapters->in_features, adapters->rank), 256);
   if (rc != GQ_OK) return rc;
@@ -248,6 +262,8 @@ int gq_adapter_grad_f16(const gq_adapters *adapters, const void *plan, int64_t r
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: in place, dx and dx_out must have the same stride", who);
   if (dx_out == x || dx_out == dy)  // (both are read again behind it)
     return gq::fail(GQ_ERR_UNSUPPORTED, "%s: dx_out must not be x or dy", who);
+  rc = gq::check_apart(who, rows, dx_out_row_stride, adapters->in_features);
+  if (rc != GQ_OK) return rc;
   rc = gq::check_workspace(who, workspace, workspace_bytes,
                            gq::adapter_grad_workspace_bytes(rows, adapters->n_adapters, adapters->in_features, adapters->out_features,
                                                             adapters->rank), 256);

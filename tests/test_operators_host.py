@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+from launch_recorder import launches
 from popxl_addons import _gq_hip
 from popxl_addons._gq_hip import GQ_ERR_BAD_SHAPE, GQ_ERR_MISALIGNED, GQ_ERR_NULL_POINTER, GQ_ERR_UNSUPPORTED
 from popxl_addons.layers.linear_gq import LinearGQ
@@ -283,3 +284,33 @@ def test_attention_apart_from_its_queries():
         message = _refused(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16", _address(cache), _address(batch), 16, 256, 64, 16, token_stride, head_stride,
                            4, 1.0, 16, 1 << 40, None)
         assert "out must not be q" in message
+
+
+def test_results_whose_rows_lie_on_each_other():
+    """A result that is one row many times (an expanded tensor) would hold whatever came last."""
+    rotary = _address(_gq_hip.Rotary(16, 1.0, 32, 0))
+    for t, o in (((64, 32), (0, 32)), ((64, 32), (32, 0)), ((0, 32), (0, 32))):
+        out = 16 if t == o else 32
+        assert "on each other" in _refused(GQ_ERR_UNSUPPORTED, "gq_rotary_f16", 16, *t, 16, rotary, 0, out, *o, 3, 2, 32, None)
+    cache, batch = _address(_gq_hip.KvCache(16, 16, 16, 16, 10, 2, 64)), _address(_gq_hip.KvBatch(16, 16, 16, 3, 4, 5))
+    for o in ((0, 64), (256, 0)):
+        assert "on each other" in _refused(GQ_ERR_UNSUPPORTED, "gq_kv_attention_f16", cache, batch, 16, 256, 64, 32, *o, 4, 1.0, 16, 1 << 40, None)
+    adapters = _address(_gq_hip.Adapters(16, 16, 16, 4, 8, 64, 128))
+    for stride in (0, 120):
+        assert "on each other" in _refused(GQ_ERR_UNSUPPORTED, "gq_adapter_apply_f16", adapters, 16, 5, 16, 64, 16, 128, 32, stride, 0, 256, 1 << 40, None)
+    for stride in (0, 63):
+        assert "on each other" in _refused(GQ_ERR_UNSUPPORTED, "gq_adapter_grad_f16", adapters, 16, 5, 16, 64, 16, 128, 64, 64, 32, stride, 16, 16, 256,
+                                           1 << 40, None)
+    k = _address(_gq_hip.KvCache(16, 16, 16, 16, 10, 2, 64))
+    assert "on each other" in _refused(GQ_ERR_UNSUPPORTED, "gq_kv_gather_f16", k, batch, 16, 16, None)
+
+
+def test_strides_of_single_rows_do_not_matter():
+    fake = 1 << 20
+    cache = ["KvCache", fake, fake, fake, fake, 10, 2, 64]
+    calls = [[0, "gq_rotary_f16", [fake, 0, 32, fake, ["Rotary", fake, 1.0, 32, 0], 0, 2 * fake, 0, 32, 1, 2, 32, None]],
+             [0, "gq_rotary_f16", [fake, 32, 0, fake, ["Rotary", fake, 1.0, 32, 0], 0, 2 * fake, 32, 0, 5, 1, 32, None]],
+             [0, "gq_kv_attention_f16", [cache, ["KvBatch", fake, fake, fake, 1, 4, 1], fake, 0, 64, 2 * fake, 0, 64, 2, 1.0, fake, 1 << 40, None]],
+             [0, "gq_adapter_apply_f16", [["Adapters", fake, fake, fake, 4, 8, 64, 128], fake, 1, fake, 64, fake, 128, 2 * fake, 0, 0, fake, 1 << 40, None]]]
+    for call, result in zip(calls, launches(calls)):
+        assert result["code"] == 0 and result["records"], call
