@@ -207,6 +207,8 @@ __global__ __launch_bounds__(kSize) void kv_append_kernel(AppendArgs a) {
       if (frexpf(need / old, &e) == 0.5f) --e;
       scale = ldexpf(old, e);
       shrink = ldexpf(1.f, -e);
+    } else if (old == 0.f && p.slot > 0) {
+      shrink = 0.f;  // tokens under a scale of 0 are zeros whatever their codes (a cache made elsewhere), and stay it
     }
   }
   if (tid == 0 && (scale != old || p.slot == 0)) *scale_at = scale;

@@ -41,7 +41,8 @@ class KVCacheGQ:
 
     @classmethod
     def from_tensors(cls, k_codes, v_codes, k_scale, v_scale):
-        """A cache on tensors that exist (not copied).  Scales are not negative."""
+        """A cache on tensors that exist (not copied).  Scales are not negative; tokens under a scale of 0 are zeros, whatever
+        their codes."""
         import torch
 
         self = cls.__new__(cls)

@@ -352,3 +352,27 @@ def test_nothing_to_do(hip, device):
         batch = _int32(device, [0, 1, 3], [9, 100], table)
         kv_cache_append(cache, q, q, *batch)
         assert (kv_cache_attention(q, cache, *batch) == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_codes_under_a_scale_of_zero_are_zeros(hip, device, new):
+    """Tokens under a scale of 0 have the value 0 whatever their codes (a cache made elsewhere), and keep it when later tokens of
+    their block bring a scale."""
+    dim, heads, before = 64, 2, 10
+    rng = np.random.default_rng(3)
+    codes = [torch.from_numpy(rng.integers(1, 256, shape).astype(np.uint8)).to(device) for shape in ((2, heads, BLOCK, dim), (2, heads, dim, BLOCK))]
+    scale = torch.tensor([[0.0, 0.5], [0.25, 0.0]], dtype=torch.float32, device=device)
+    cache = KVCacheGQ.from_tensors(*codes, scale.clone(), scale.flip(1).contiguous())
+    table = [[0], [1]]
+    batch = _int32(device, [0, before, 2 * before], [before, before], table)
+    values = [t.clone() for t in kv_cache_gather(cache, *batch, tokens=2 * before)]
+    for i, t in enumerate(values):
+        assert (t[:before, i] == 0).all() and (t[before:, 1 - i] == 0).all() and (t[:before, 1 - i] != 0).any()
+    k, v = (torch.from_numpy(_normal(j, 2 * new, heads, dim)).to(device) for j in (1, 2))
+    kv_cache_append(cache, k, v, *_int32(device, [0, new, 2 * new], [before + new] * 2, table))
+    after = kv_cache_gather(cache, *_int32(device, [0, before + new, 2 * (before + new)], [before + new] * 2, table), tokens=2 * (before + new))
+    for i, (old, got, x) in enumerate(zip(values, after, (k, v))):
+        for b in range(2):
+            there = got[b * (before + new):][:before + new]
+            assert torch.equal(there[:before], old[b * before:][:before]), (i, b)  # (values of +-4 at most: scales of 0.25 and 0.5 do not grow)
+            assert (there[before:] - x[b * new:][:new]).abs().max() <= 0.5
