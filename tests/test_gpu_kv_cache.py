@@ -376,3 +376,46 @@ def test_codes_under_a_scale_of_zero_are_zeros(hip, device, new):
             there = got[b * (before + new):][:before + new]
             assert torch.equal(there[:before], old[b * before:][:before]), (i, b)  # (values of +-4 at most: scales of 0.25 and 0.5 do not grow)
             assert (there[before:] - x[b * new:][:new]).abs().max() <= 0.5
+
+
+MIXED = [[64] + [1] * 40, [1] * 8, [3, 64, 17, 0, 130] + [1] * 90, [20, 2] + [1] * 20]  # few tokens a sequence on average, not in every block
+
+
+@pytest.mark.parametrize("heads,dim", [(2, 64), (1, 256)])
+@pytest.mark.parametrize("fresh", MIXED, ids=len)
+def test_append_codes_of_mixed_batches(hip, device, heads, dim, fresh):
+    """Batches of few new tokens a sequence whose blocks get from one token to all 64: codes and scales bit for bit."""
+    before = np.random.default_rng(len(fresh)).integers(0, 100, len(fresh))
+    lengths = before + fresh
+    table, n_blocks = _table(lengths, dim)
+    cache, plain = KVCacheGQ(n_blocks, heads, dim, device), PlainCache(n_blocks, heads, dim)
+    for i, (step, length) in enumerate(((before, before), (np.array(fresh), lengths))):
+        offsets = np.concatenate([[0], np.cumsum(step)])
+        k, v = (_normal(10 * i + j, offsets[-1], heads, dim) * np.float16([1, 3][i]) for j in range(2))
+        kv_cache_append(cache, torch.from_numpy(k).to(device), torch.from_numpy(v).to(device), *_int32(device, offsets, length, table))
+        plain.append(k, v, offsets, length, table)
+    got = _codes(cache)
+    for b, n in enumerate(lengths):
+        for p in range(-(-n // BLOCK)):
+            block, slots = table[b, p], min(BLOCK, n - p * BLOCK)
+            for j in range(2):
+                assert np.array_equal(got[2 + j][block], plain.scale[j][block]), (b, p, "kv"[j], "scale")
+                assert np.array_equal(got[j][block][:, :slots], plain.codes[j][block][:, :slots]), (b, p, "kv"[j])
+
+
+@pytest.mark.parametrize("layout,rotary_dim,dim", [("half", 256, 256), ("interleaved", 256, 256), ("half", 160, 256), ("interleaved", 200, 208),
+                                                   ("half", 64, 64), ("interleaved", 8, 16)])
+@pytest.mark.parametrize("fresh", MIXED, ids=len)
+def test_append_with_rotary_of_mixed_batches(hip, device, layout, rotary_dim, dim, fresh):
+    """The same with keys turned on the way, more pairs than a wave has lanes among them: the bits of turning them first."""
+    lengths = np.random.default_rng(len(fresh)).integers(0, 100, len(fresh)) + fresh
+    table, n_blocks = _table(lengths, 5)
+    batch = _int32(device, np.concatenate([[0], np.cumsum(fresh)]), lengths, table)
+    k, v = (torch.from_numpy(_normal(j, sum(fresh), 2, dim)).to(device) for j in range(2))
+    rotary = RotaryPosEmbed(rotary_dim, layout=layout, device=device)
+    one, two = (KVCacheGQ(n_blocks, 2, dim, device) for _ in range(2))
+    positions = np.concatenate([np.arange(n - f, n) for n, f in zip(lengths, fresh)])
+    kv_cache_append(one, k, v, *batch, rotary=rotary)
+    kv_cache_append(two, rotary_pos_embed(k, *_int32(device, positions), rotary), v, *batch)
+    for a, b in zip(_codes(one), _codes(two)):
+        assert np.array_equal(a, b)
