@@ -24,7 +24,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None):
         linear  w / s (positions interpolated)
         ntk     base * s^(r / (r - 2)): the slowest pair is stretched by s, the fastest hardly at all
         yarn    pairs that turn more than beta_fast (32) times in original_length keep w, those that turn less than beta_slow (1)
-                times get w / s, with a ramp in between; factor 0.1 ln s + 1 (https://arxiv.org/abs/2309.00071)
+                times get w / s; in between (turns - beta_slow) / (beta_fast - beta_slow) of w stays, as the paper has it
+                (https://arxiv.org/abs/2309.00071): linear in the turns, not in the number of the pair between two corners.  A model
+                that was tuned with another ramp needs its own frequencies (RotaryPosEmbed.from_frequencies); factor 0.1 ln s + 1
     """
     if rotary_dim < 2 or rotary_dim % 2 != 0:
         raise ValueError(f"rotary_dim={rotary_dim} must be even and positive")
@@ -63,17 +65,32 @@ class RotaryPosEmbed:
     rotary_dim are left as they are."""
 
     def __init__(self, rotary_dim, base=10000.0, layout="interleaved", scaling=None, device="cuda"):
+        self._adopt(*rotary_frequencies(rotary_dim, base, scaling), layout, device)
+
+    @classmethod
+    def from_frequencies(cls, frequencies, factor=1.0, layout="interleaved", device="cuda"):
+        """Frequencies that were made elsewhere (host values): radians a position of every pair [rotary_dim / 2], and the factor of the turned
+        values."""
+        self = cls.__new__(cls)
+        frequencies = np.asarray(frequencies)
+        if frequencies.ndim != 1 or len(frequencies) == 0 or frequencies.dtype.kind not in "fiu" or not np.isfinite(frequencies).all():
+            raise ValueError("RotaryPosEmbed: frequencies must be one finite number for each pair")
+        if not math.isfinite(factor):
+            raise ValueError(f"RotaryPosEmbed: factor={factor} must be finite")
+        self._adopt(frequencies.astype(np.float64), float(factor), layout, device)
+        return self
+
+    def _adopt(self, frequencies, factor, layout, device):
         import torch
 
         if layout not in _LAYOUTS:
             raise ValueError(f"unknown rotary layout {layout!r}; expected one of {sorted(_LAYOUTS)}")
-        if rotary_dim > 256:
-            raise ValueError(f"rotary_dim={rotary_dim} exceeds 256")
-        frequencies, self.factor = rotary_frequencies(rotary_dim, base, scaling)
-        self.rotary_dim, self.layout = rotary_dim, layout
+        self.rotary_dim, self.factor, self.layout = 2 * len(frequencies), factor, layout
+        if self.rotary_dim > 256:
+            raise ValueError(f"rotary_dim={self.rotary_dim} exceeds 256")
         self.turns = torch.from_numpy(frequencies / (2 * math.pi)).to(device)
         self.index = self.turns.get_device()
-        self._c = _gq_hip.Rotary(self.turns.data_ptr(), self.factor, rotary_dim, _LAYOUTS[layout])
+        self._c = _gq_hip.Rotary(self.turns.data_ptr(), factor, self.rotary_dim, _LAYOUTS[layout])
 
     @property
     def argument(self):

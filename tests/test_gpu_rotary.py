@@ -126,3 +126,14 @@ def test_most_tokens(hip, device, dim, tokens):
         assert torch.equal(got[i:i + third], rotary_pos_embed(t[i:i + third], positions[i:i + third], rotary)), i
     assert rotary_pos_embed(t, positions, rotary, out=t) is t
     assert torch.equal(got, t)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_given_frequencies(hip, device, layout):
+    t, positions = _rows(9, 3, 80, 4), np.array([0, 1, -7, 100, 2047, 65536, 3, 2 ** 31 - 1, -2 ** 31])
+    w = np.random.default_rng(1).normal(0, 1, 32)
+    got = rotary_pos_embed(torch.from_numpy(t).to(device), torch.tensor(positions, dtype=torch.int32, device=device),
+                           RotaryPosEmbed.from_frequencies(w, 1.25, layout=layout, device=device)).cpu().numpy()
+    turns = positions[:, None] * (w / (2 * np.pi))  # (reduced to a turn as the definition does, so that far positions mean the same)
+    want, room = zip(*(rotate(t[i:i + 1], [1], 2 * np.pi * (turns[i] - np.rint(turns[i])), 1.25, layout) for i in range(len(t))))
+    assert_within(got, np.concatenate(want), np.concatenate(room))

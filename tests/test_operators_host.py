@@ -314,3 +314,34 @@ def test_strides_of_single_rows_do_not_matter():
              [0, "gq_adapter_apply_f16", [["Adapters", fake, fake, fake, 4, 8, 64, 128], fake, 1, fake, 64, fake, 128, 2 * fake, 0, 0, fake, 1 << 40, None]]]
     for call, result in zip(calls, launches(calls)):
         assert result["code"] == 0 and result["records"], call
+
+
+def test_rotary_of_given_frequencies():
+    """Frequencies of the caller's own (another way to stretch a context, say) instead of base and scaling."""
+    w, factor = rotary_frequencies(64, base=500.0, scaling=dict(kind="yarn", factor=8, original_length=4096))
+    made = RotaryPosEmbed(64, base=500.0, layout="half", scaling=dict(kind="yarn", factor=8, original_length=4096), device="cpu")
+    for frequencies in (w, w.tolist(), torch.from_numpy(w)):
+        given = RotaryPosEmbed.from_frequencies(frequencies, factor, layout="half", device="cpu")
+        assert torch.equal(given.turns, made.turns) and (given.rotary_dim, given.factor, given.layout) == (64, made.factor, "half")
+        assert bytes(given._c)[8:] == bytes(made._c)[8:]
+    single = RotaryPosEmbed.from_frequencies(np.float32([0.5, -0.25, 0]), device="cpu")  # backwards, and not at all
+    assert single.turns.dtype == torch.float64 and np.array_equal(single.turns.numpy() * 2 * math.pi, [0.5, -0.25, 0]) and single.factor == 1
+    for bad in ([], [[1.0, 2.0]], 1.0, [1.0] * 129, [1.0, math.nan], [math.inf], [1j]):
+        with pytest.raises(ValueError):
+            RotaryPosEmbed.from_frequencies(bad, device="cpu")
+    for factor in (math.nan, math.inf):
+        with pytest.raises(ValueError):
+            RotaryPosEmbed.from_frequencies([1.0], factor, device="cpu")
+    with pytest.raises(ValueError):
+        RotaryPosEmbed.from_frequencies([1.0], layout="other", device="cpu")
+
+
+def test_yarn_ramp_is_linear_in_turns():
+    """Between the pairs that are kept and those that are stretched: (turns - beta_slow) / (beta_fast - beta_slow) is what stays of w."""
+    w, _ = rotary_frequencies(128, base=1e6)
+    for fast, slow in ((32, 1), (20, 4)):
+        yarn, _ = rotary_frequencies(128, base=1e6, scaling=dict(kind="yarn", factor=4, original_length=2048, beta_fast=fast, beta_slow=slow))
+        for i in range(64):
+            turns = 2048 * w[i] / (2 * math.pi)
+            stays = min(max((turns - slow) / (fast - slow), 0), 1)
+            assert math.isclose(yarn[i], w[i] * stays + w[i] / 4 * (1 - stays), rel_tol=1e-14)
