@@ -420,7 +420,8 @@ int gq_compress_f32(const float *t, uint16_t *packed, uint16_t *scale, uint16_t 
  *   t, out     [tokens, heads, head_dim] binary16, the last axis contiguous, strides in elements; out may be t (same strides),
  *              other overlaps are the caller's error
  *   positions  [tokens] int32;  turns [rotary_dim / 2] binary64
- * rotary_dim is even and <= 256.  The fast kernel needs 16-byte aligned rows (strides and head_dim % 8 == 0) and rotary_dim % 8
+ * rotary_dim is even and <= 256, head_dim <= 2048, 2^24 tokens (two launches above 2^23).  A result whose rows lie on each other (a
+ * stride of 0) is refused, here and below.  The fast kernel needs 16-byte aligned rows (strides and head_dim % 8 == 0) and rotary_dim % 8
  * (interleaved) or % 16 (half); others run element by element with the same results.
  */
 #define GQ_ROTARY_INTERLEAVED 0
@@ -437,8 +438,8 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
 
 /*
  * 8-bit key/value cache in blocks of GQ_KV_BLOCK tokens, one binary32 scale for the keys and one for the values of each
- * (block, head); value = (byte - 128) * scale, bytes 1 ... 255, scales not negative.  head_dim is a multiple of 16, at most 256; the code arrays are
- * 16-byte aligned.
+ * (block, head); value = (byte - 128) * scale, bytes 1 ... 255, scales not negative (0: zeros, whatever the bytes).  head_dim is a
+ * multiple of 16, at most 256; the code arrays are 16-byte aligned.
  *
  * A batch is B sequences.  Rows offsets[b] ... offsets[b + 1] - 1 of the row tensors (k, v, q, out) are the newest tokens of
  * sequence b, seq_lens[b] its length with them: its last row has position seq_lens[b] - 1.  A sequence that is given more rows
@@ -453,10 +454,10 @@ int gq_rotary_f16(const uint16_t *t, int64_t t_token_stride, int64_t t_head_stri
  *   does).  A block that starts with these tokens gets scale amax / 127; in one that has tokens the scale grows, where it
  *   must, by a power of two and the codes there are scaled down by it: |value - x| < scale always.  A value that is not
  *   finite makes all values of its (block, head) not finite.
- * gq_kv_gather_f16     the values of the batch's rows, [tokens, kv_heads, head_dim] binary16, contiguous, 16-byte aligned.
+ * gq_kv_gather_f16     the values of the batch's rows, [tokens, kv_heads, head_dim] binary16, contiguous, 16-byte aligned, apart.
  * gq_kv_attention_f16  out[row][head] = softmax(scale q . k) v over the tokens at the row's position and before, query head i
  *   with kv head i / (q_heads / kv_heads).  q, out [tokens, q_heads, head_dim]: q strides multiples of 8 and 16-byte aligned,
- *   out any strides (elements), apart from q.  Binary32 softmax and sums; probabilities enter the product with the values as binary16.
+ *   out any strides (elements), apart from q (out == q is refused).  Binary32 softmax and sums; probabilities enter the product with the values as binary16.
  *   workspace: gq_kv_attention_workspace_bytes() bytes, 16-byte aligned, any contents, not shared by calls that may overlap.
  */
 #define GQ_KV_BLOCK 64

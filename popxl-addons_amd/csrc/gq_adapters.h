@@ -7,7 +7,6 @@ namespace gq {
 constexpr int kAdapterSmallTile = 16, kAdapterLargeTile = 64;  // rows of one adapter that a workgroup takes together
 constexpr int kAdapterSegment = 2048;                          // rows that one part of a weight gradient sums over
 constexpr int kMostAdapters = 2048;
-constexpr int64_t kMostAdapterRows = (int64_t)1 << 24;
 
 struct AdapterTile {
   int adapter;  // -1: rows without one

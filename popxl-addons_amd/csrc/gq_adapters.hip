@@ -124,8 +124,8 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
     }
     if (tid == 0 && i > 0) a.plan[a.counts + i - 1] = all;
   }
-  // Parts are numbered like segments; an adapter of one segment leaves its number unused.  The numbers are compact enough:
-  // only those of adapters with several segments are used, so they are counted apart.
+  // Parts: the segments of adapters that have several, in the same order, counted apart (an adapter of one segment writes
+  // its gradient itself).
   __syncthreads();
   int several = 0;
 #pragma unroll
@@ -806,7 +806,8 @@ int64_t down_splits(int64_t tiles, int64_t features) {
 
 // As many workgroups as are resident together, no more: each sums its tile's v anew, and a few behind the others cost as much as
 // a whole turn of them (6001 rows to 12288, rank 32, 376 tiles: 2, 3, 6 ranges 74, 80, 77 us; 8192 rows to 4096, rank 64, 128
-// tiles: 4, 8 ranges 43, 52 us; 150 rows to 16384, rank 64: 13, 16, 32 ranges 27, 24, 29 us).  `tiles` counts
+// tiles: 4, 8 ranges 43, 52 us; 150 rows to 16384, rank 64: 13, 16, 32 ranges 27, 24, 29 us).  It is a whole number, so a few
+// tiles more can halve the workgroups: 4096 to 4096, rank 16, 8180 rows, 532, 542, 557, 602 tiles: 63, 65, 73, 71 us.  `tiles` counts
 // the last one of every adapter: an eighth of them may be nobody's.
 int64_t up_ranges(int64_t tiles, int64_t rank, bool large) {
   const int64_t resident = large || rank > 64 ? 512 : 1024, ranges = (resident + tiles / 8) / tiles;

@@ -29,7 +29,7 @@ int check_kv(const char *who, const gq_kv_cache *cache, const gq_kv_batch *batch
     return fail(GQ_ERR_BAD_SHAPE, "%s: negative size", who);
   if (cache->head_dim % 16 != 0 || cache->head_dim < 16 || cache->head_dim > 256)
     return fail(GQ_ERR_UNSUPPORTED, "%s: head_dim=%d must be a multiple of 16 up to 256", who, cache->head_dim);
-  // (grid dimensions: heads in y; sequences and rows in x)
+  // (what the kernels count in 31 bits; whether a batch of these sizes fits a grid is seen to by the launchers)
   if (cache->n_blocks > kLargest || cache->kv_heads > 1024 || batch->sequences > (1 << 20) || batch->table_width > (1 << 24) ||
       batch->tokens > (1 << 24))
     return fail(GQ_ERR_UNSUPPORTED,

@@ -691,6 +691,8 @@ int launch_kv_attention(const KvCache &cache, const KvBatch &batch, const uint16
   // costs what kv_split_kernel takes for 16 to 32.  Measured at 32 rows 66 us by kv_split_kernel and 160 us by
   // kv_tile_kernel (8 sequences of up to 3000, 16 heads of 256), 67 and 94 (32 of up to 3000, 8 heads of 128), at 64
   // rows 49 and 49 (one of 4000, 16 heads of 256) and 105 and 95 (32 of up to 3000, 8 heads of 128), at 256 rows 90 and 52.
+  // A batch of both kinds goes to one of them: 64 single tokens over up to 32768 beside a prompt of 1024, 32 / 8 heads of 128, take
+  // 902 us, as two calls 383 + 40; 64 over up to 2048 beside a prompt of 2048, 16 heads of 256, 561 us, as two calls 201 + 112.
   // (The units of kv_split_kernel have to be countable in 31 bits.)
   const double most_units = (double)cache.heads * ((double)batch.tokens * a.group / kRows + batch.sequences) * (batch.width + 1);
   if (most_units >= 2147483648. || (int64_t)batch.tokens * a.group >= (int64_t)kTileLeast * batch.sequences)

@@ -2,7 +2,7 @@
 //
 // Quantisation.  A block that starts with these tokens takes scale = amax / 127.  A block that has tokens keeps its scale s
 // where amax / 127 <= s; otherwise s grows by the least power of two that covers the new tokens and the codes that are there
-// are scaled down by it (rint).  Growth by powers of two bounds what repeated rounding can add up to: a code is rounded by at
+// are scaled down by it (rint), or, under a scale of 0, cleared.  Growth by powers of two bounds what repeated rounding can add up to: a code is rounded by at
 // most 1/2 of its own step, then by 1/2 of each later step, and the steps at least double: |value - x| < s (1/2 + 1/4 + ...)
 // < s.  (With s following amax / 127 itself, every token that sets a new maximum would add another half step.)
 // Codes are rint(x / s) with the correctly rounded quotient: a plain binary32 program gets the same codes.
@@ -67,7 +67,7 @@ typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 
 // What turns values into codes at one scale: rint of the correctly rounded binary32 quotient.  The product with the reciprocal
 // is within 3 2^-24 |q| <= 2.3e-5 of that quotient, so it rounds to the same integer unless it is nearer than that to a tie;
-// then (one group of 512 values in 60) the quotients are taken in binary64.  That is exact: the product with the binary64
+// then (of normal binary16 values one wave's 512 in 11 to 14, exact ties among them) the quotients are taken in binary64.  That is exact: the product with the binary64
 // reciprocal is within 2^-52 of x / s, relatively, and a quotient of an 11-bit and a 24-bit number is never half way between
 // two binary32 numbers (25 bits) nor nearer to that than 2^-49, so rounding the product rounds the quotient.
 struct Coder {

@@ -170,11 +170,13 @@ def kv_cache_attention(q, cache, offsets, seq_lens, block_table, scale=None, out
             i // (q_heads / kv_heads)
         offsets, seq_lens, block_table: the batch (see the module)
         scale (float): of the scores, head_dim ** -0.5 if None
-        out (torch.Tensor): float16, the shape of q, apart from it; a new tensor if None, whose rows from offsets[B] on hold
-            nothing in particular
+        out (torch.Tensor): float16, the shape of q, apart from it (q itself is refused); a new tensor if None, whose rows from
+            offsets[B] on hold nothing in particular
 
     Returns:
-        torch.Tensor: `out`.  Decode steps, prompts in chunks and mixtures of both are one call; results do not depend on timing.
+        torch.Tensor: `out`.  Decode steps, prompts in chunks and mixtures of both are one call; results do not depend on timing.  (One
+        kernel takes the whole batch, chosen by its rows a sequence on average: decode steps with long histories beside a long chunk
+        take about half the time as two calls.)
     """
     import torch
 
