@@ -103,6 +103,12 @@ class LinearGQ:
             self._decode_copy = None
             self.prepack_for_decode()
 
+    def _check_device(self, name, t):
+        """(A kernel on the device of `t` would read addresses of another one, or of the host.)"""
+        device = self.variables.weight_compressed.data.device
+        if t.device != device:
+            raise ValueError(f"LinearGQ: {name} is on {t.device}, the layer is on {device}")
+
     # --------------------------------------------------------------------------------- build
 
     def build(self, x, activation=None, adapters=None, plan=None):
@@ -134,6 +140,7 @@ class LinearGQ:
         packed_shape, _ = self._variable_shapes(in_features)
         if v.weight_compressed.shape != packed_shape:
             raise ValueError(f"LinearGQ: x has {in_features} features but weight_compressed is {v.weight_compressed.shape}")
+        self._check_device("x", x)
         b = v.bias.data if self.bias else None
 
         # A decode batch that is a column slice of a wider matrix (part of the output of fused projections, say)
@@ -205,6 +212,7 @@ class LinearGQ:
             raise ValueError(f"LinearGQ.grad: dy has {dy.shape[-1]} features, the layer {self.out_features}")
         if (adapters is None) != (plan is None) or (adapters is None) != (x is None):
             raise ValueError("LinearGQ.grad: x, adapters and plan go together")
+        self._check_device("dy", dy)
         rows, n_groups, _ = v.weight_compressed.shape
         in_features = n_groups * self.group_size if self.dim == 0 else rows
         if adapters is not None and (adapters.in_features, adapters.out_features) != (in_features, self.out_features):

@@ -345,3 +345,33 @@ def test_yarn_ramp_is_linear_in_turns():
             turns = 2048 * w[i] / (2 * math.pi)
             stays = min(max((turns - slow) / (fast - slow), 0), 1)
             assert math.isclose(yarn[i], w[i] * stays + w[i] / 4 * (1 - stays), rel_tol=1e-14)
+
+
+class _Placed(torch.Tensor):
+    """A host tensor that says it lies on the GPU `index`."""
+
+    index = 0
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", self.index))
+
+    def get_device(self):
+        return self.index
+
+
+class _PlacedElsewhere(_Placed):
+    index = 1
+
+
+@pytest.mark.parametrize("dim", [0, -1])
+def test_layer_on_another_device_than_its_input(dim):
+    """The kernels would read the weight's address on the input's device."""
+    layer = LinearGQ(64, group_size=32, dim=dim)
+    layer.init_variables(64, torch.float16, "cpu")
+    x = torch.zeros((3, 64), dtype=torch.float16).as_subclass(_Placed)
+    for where in ("cpu", "cuda:1"):
+        if where != "cpu":
+            for name in ("weight_compressed", "weight_decompression_scale", "weight_decompression_bias", "bias"):
+                layer.variables[name].data = layer.variables[name].data.as_subclass(_PlacedElsewhere)
+        for call in (layer.build, layer.grad):
+            with pytest.raises(ValueError, match=f"the layer is on {where}"):
+                call(x)
