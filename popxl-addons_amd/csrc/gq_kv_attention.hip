@@ -589,7 +589,9 @@ __global__ __launch_bounds__(kThreads) void kv_join_kernel(AttentionArgs a) {
   const uint32_t from = base + which * shape.blocks, to = from + shape.blocks;
   if (unit == from || cut.start(w - 1) > from) return;
   const int h = which / shape.tiles, tile = which - h * shape.tiles;
-  const int first = w - 1, last = cut.owner(to - 1);
+  // (the last group at most: where offsets that do not ascend make 2^32 units or more, their number wraps, and a tile's units may
+  // end behind it)
+  const int first = w - 1, last = min(cut.owner(to - 1), cut.groups - 1);
   const int here = min(kRows, s.count * a.group - tile * kRows), d = lane * 4;
   const float *stats = a.parts + (int64_t)2 * a.groups * kRows * dim;
   // a wave has a row, or, of few rows, every fourth part of each

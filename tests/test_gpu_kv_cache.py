@@ -419,3 +419,28 @@ def test_append_with_rotary_of_mixed_batches(hip, device, layout, rotary_dim, di
     kv_cache_append(two, rotary_pos_embed(k, *_int32(device, positions), rotary), v, *batch)
     for a, b in zip(_codes(one), _codes(two)):
         assert np.array_equal(a, b)
+
+
+def test_offsets_that_do_not_ascend(hip, device):
+    """What rows then hold is not said; they stay rows of the tensors, blocks stay blocks of the cache and parts stay parts of the
+    workspace, also where the units of all sequences are more than 32 bits count."""
+    heads, dim = 1, 16
+    cache, plain, table = _filled(device, [100, 30], heads, dim, 61)
+    good = _int32(device, [0, 1, 4], [100, 30], table)
+    q = torch.from_numpy(_normal(5, 4, heads, dim)).to(device)
+    want = kv_cache_attention(q, cache, *good)
+    for offsets in ([4, 0, 4], [-5, 9, 2], [2 ** 31 - 1, -2 ** 31, 3], [3, 2, 1]):
+        batch = _int32(device, offsets, [100, 30], table)
+        kv_cache_append(KVCacheGQ(5, heads, dim, device), q, q, *batch)
+        kv_cache_gather(cache, *batch, tokens=4)
+        kv_cache_attention(q, cache, *batch)
+    # 512 sequences that are each given all 16384 rows (1024 tiles) over 8192 blocks, 2^32 units, and one with few more
+    rows, blocks, many = 16384, 8192, 512
+    wide = torch.full((2 * many + 1, blocks), -1, dtype=torch.int32, device=device)  # (no block is there)
+    q2 = torch.zeros((rows, heads, dim), dtype=torch.float16, device=device)
+    for extra in (0, 7, 2000):
+        offsets = [0, rows] * many + [0, 16 if extra else 0]
+        lengths = [blocks * BLOCK] * 2 * many + [extra * BLOCK]
+        assert kv_cache_attention(q2, cache, *_int32(device, offsets, lengths), wide).shape == q2.shape
+    torch.cuda.synchronize()
+    assert torch.equal(kv_cache_attention(q, cache, *good), want)
