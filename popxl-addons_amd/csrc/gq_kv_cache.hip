@@ -72,7 +72,8 @@ typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 // two binary32 numbers (25 bits) nor nearer to that than 2^-49, so rounding the product rounds the quotient.
 struct Coder {
   float scale, inverse;
-  __device__ explicit Coder(float s) : scale(s), inverse(s > 0.f && s < __builtin_inff() ? 1.f / s : 0.f) {}
+  // (the least scale of a value is 2^-24 / 127; a smaller one, from elsewhere, has only zeros to code, and may have no reciprocal)
+  __device__ explicit Coder(float s) : scale(s), inverse(s > 1e-30f && s < __builtin_inff() ? 1.f / s : 0.f) {}
   __device__ uint2_t operator()(half8_t x) const {
     uint2_t word = {0x80808080u, 0x80808080u};
     if (inverse == 0.f) return word;  // a block of zeros, or one that is not finite (its scale says so)
@@ -203,8 +204,10 @@ __global__ __launch_bounds__(kSize) void kv_append_kernel(AppendArgs a) {
   if (!(need <= old) && old == old) {  // (a scale that is NaN stays)
     scale = need;
     if (old > 0.f && need < __builtin_inff()) {
-      int e;
-      if (frexpf(need / old, &e) == 0.5f) --e;
+      // (by mantissas and exponents: the quotient of a scale of 1e-40, which a cache made elsewhere may have, is infinite)
+      int e_need, e_old;
+      const float m_need = frexpf(need, &e_need), m_old = frexpf(old, &e_old);
+      const int e = e_need - e_old + (m_need > m_old ? 1 : 0);
       scale = ldexpf(old, e);
       shrink = ldexpf(1.f, -e);
     } else if (old == 0.f && p.slot > 0) {

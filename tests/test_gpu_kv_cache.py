@@ -444,3 +444,26 @@ def test_offsets_that_do_not_ascend(hip, device):
         assert kv_cache_attention(q2, cache, *_int32(device, offsets, lengths), wide).shape == q2.shape
     torch.cuda.synchronize()
     assert torch.equal(kv_cache_attention(q, cache, *good), want)
+
+
+@pytest.mark.parametrize("old", [1e-45, 1e-42, 1e-38, 1e-36, 2.0 ** -126, 3e-31, 4.7e-10, 1e-3])
+@pytest.mark.parametrize("new", [1, 40])
+def test_growth_from_small_scales(hip, device, old, new):
+    """The least power of two, however far below the new tokens the scale is (a cache made elsewhere), and zeros under it."""
+    dim, before = 64, 7
+    old = np.float32(old)
+    for x in (_normal(5, new, 1, dim), np.zeros((new, 1, dim), np.float16)):
+        codes = [torch.from_numpy(np.random.default_rng(j).integers(1, 256, (1, 1, *s)).astype(np.uint8)).to(device) for j, s in enumerate(((BLOCK, dim), (dim, BLOCK)))]
+        cache = KVCacheGQ.from_tensors(*codes, *(torch.full((1, 1), float(old), dtype=torch.float32, device=device) for _ in range(2)))
+        had = _codes(cache)
+        part = torch.from_numpy(x).to(device)
+        kv_cache_append(cache, part, part, *_int32(device, [0, new], [before + new], [[0]]))
+        got, need = _codes(cache), np.abs(x).max().astype(np.float32) / np.float32(127)
+        e = 0
+        while np.ldexp(np.float64(old), e) < need:
+            e += 1
+        scale = np.float32(np.ldexp(np.float64(old), e))
+        for j in range(2):
+            assert got[2 + j][0, 0] == scale
+            assert np.array_equal(got[j][0, 0, before:before + new], np.clip(np.rint(x[:, 0].astype(np.float32) / scale), -127, 127))
+            assert np.array_equal(got[j][0, 0, :before], np.rint(had[j][0, 0, :before] * 2.0 ** -e))
