@@ -455,8 +455,10 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
         for (int i = 0; i < 16; ++i) top = fmaxf(top, score[T][i]);
       top = fmaxf(top, __shfl_xor(top, 32)) * factor;
       const bool raise = top > most + 8.f || (most == -__builtin_inff() && top > most);
-      // the value scale against its reference
-      const bool scaled = value_scale > 0.f && value_scale < __builtin_inff();
+      // the value scale against its reference.  Values under a scale below 1e-12 are nothing to a binary16 result (2e-10 at most, half
+      // its smallest number is 3e-8), and the accumulators need not hold what its ratio to another scale makes of them; the
+      // append makes no scale below 2^-24 / 127.
+      const bool nothing = value_scale < 1e-12f, scaled = !nothing && value_scale < __builtin_inff();
       const bool turn = scaled && (fresh || value_scale > 16.f * reference || value_scale * 16.f < reference);
       if (__builtin_expect(!again && (turn || __any(raise)), 0)) {
         const float next = raise ? top : most;
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
         most = next;
         sum *= keep;
         if (turn) {
-          if (!fresh) keep *= reference / value_scale;
+          if (!fresh) keep *= fminf(reference / value_scale, 3e38f);
           reference = value_scale, fresh = false;
         }
         if (block > first_block) {
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
           break;
         }
       }
-      const float ratio = value_scale == 0.f ? 1.f : value_scale / reference, share = none ? 1.f : ratio;
+      const float ratio = nothing ? 1.f : value_scale / reference, share = none ? 1.f : ratio;
       const float shift = __builtin_amdgcn_logf(share) - (most == -__builtin_inff() ? 0.f : most);
       half8_t pf[2][2];
       float part = 0.f;
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(kTileThreads, DP > 128 ? 1 : 2) void kv_tile_kernel
           pf[T][i >> 3][i & 7] = (half_t)p;
         }
       sum += part / share;
-      if (value_scale == 0.f) {  // (values of scale 0 are zeros, whatever their codes)
+      if (nothing) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) pf[T][0] = pf[T][1] = half8_t{};
       }

@@ -467,3 +467,19 @@ def test_growth_from_small_scales(hip, device, old, new):
             assert got[2 + j][0, 0] == scale
             assert np.array_equal(got[j][0, 0, before:before + new], np.clip(np.rint(x[:, 0].astype(np.float32) / scale), -127, 127))
             assert np.array_equal(got[j][0, 0, :before], np.rint(had[j][0, 0, :before] * 2.0 ** -e))
+
+
+@pytest.mark.parametrize("fresh", [1, 70])
+@pytest.mark.parametrize("order", [(0.02, 1e-40, 0.03), (1e-42, 0.05, 1e-45), (1e-33, 1e-40, 1e-36), (3e-29, 0.02, 2e-38), (1e-11, 500.0, 1e-13)])
+def test_attention_of_small_scales(hip, device, order, fresh):
+    """Scales that no binary16 token brings (a cache made elsewhere): what lies under them is next to nothing, in every order."""
+    lengths, dim = [64 * 4 + 10], 64
+    cache, plain, table = _filled(device, lengths, 2, dim, 71)
+    for j, c in enumerate((cache.k_scale, cache.v_scale)):
+        for p in range(5):
+            plain.scale[j][table[0, p]] = order[(p + j) % 3]
+        c.copy_(torch.from_numpy(plain.scale[j]).to(device))
+    q = _normal(dim, fresh, 4, dim)
+    got = kv_cache_attention(torch.from_numpy(q).to(device), cache, *_int32(device, [0, fresh], lengths, table)).cpu().numpy()
+    want, room = attend(q, plain.values(0, 0, lengths[0], table), plain.values(1, 0, lengths[0], table), lengths[0] - fresh, dim ** -0.5)
+    assert_within(got, want, room)
