@@ -231,3 +231,12 @@ def test_layer_with_adapters(hip, device, oracle, dim, rows):
     want, rooms = adapt_grad(p["x"], dy, dx.cpu().numpy(), p["down"], p["up"], p["scaling"], p["ids"])
     for g, t, room in zip((full, d_down, d_up), want, rooms):
         assert_within(g.cpu().numpy(), t, room)
+
+
+@pytest.mark.parametrize("count", [959, 960, 1019, 1023, 1024, 2048])
+def test_plans_of_many_adapters(hip, device, count):
+    """Counts of rows around the LDS that any launch may use."""
+    p = _problem(300, 24, 40, 2, count, count)
+    d, adapters, plan = _on(device, p)
+    want, room = adapt(p["x"], p["y"], p["down"], p["up"], p["scaling"], p["ids"])
+    assert_within(low_rank_adapters(d["x"], d["y"], adapters, plan).cpu().numpy(), want, room)
