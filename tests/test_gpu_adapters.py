@@ -240,3 +240,19 @@ def test_plans_of_many_adapters(hip, device, count):
     d, adapters, plan = _on(device, p)
     want, room = adapt(p["x"], p["y"], p["down"], p["up"], p["scaling"], p["ids"])
     assert_within(low_rank_adapters(d["x"], d["y"], adapters, plan).cpu().numpy(), want, room)
+
+
+def test_calls_at_once(hip, device):
+    """One plan and its adapters on two streams at once, forward and gradients, each call with a workspace of its own."""
+    p = _problem(700, 520, 640, 24, 5, 90)
+    d, adapters, plan = _on(device, p)
+    want = low_rank_adapters(d["x"], d["y"], adapters, plan), *low_rank_adapters_grad(d["x"], d["y"], adapters, plan)
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream(device=device) for _ in range(2)], []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                results.append((low_rank_adapters(d["x"], d["y"], adapters, plan), *low_rank_adapters_grad(d["x"], d["y"], adapters, plan)))
+    torch.cuda.synchronize()
+    for result in results:
+        assert all(torch.equal(a, b) for a, b in zip(result, want))

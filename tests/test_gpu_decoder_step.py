@@ -136,3 +136,46 @@ def test_captured_decode_step(hip, device, dim):
             assert torch.equal(a, b), (i, name)
     for name in ("k_codes", "v_codes", "k_scale", "v_scale"):
         assert torch.equal(getattr(eager.cache, name), getattr(graphed.cache, name)), name
+
+
+@pytest.mark.parametrize("dim", [0, -1])
+def test_two_captured_steps(hip, device, dim):
+    """Steps of two batches in graphs of their own, on one cache, the second captured replayed first and eager steps between them:
+    the bits of eager steps."""
+    eager, graphed = Decoder(device, dim, 18), Decoder(device, dim, 18)
+    rng = np.random.default_rng(19)
+    tables, lengths = [[[0, 1], [2, 3], [4, 5]], [[6, 7], [8, 9]]], [np.array([60, 3, 64]), np.array([63, 100])]
+    state = []
+    for table, n in zip(tables, lengths):
+        x0 = to_dev(rng.normal(0, 1, (n.sum(), HIDDEN)).astype(np.float16), device)
+        ids = list(range(len(n)))
+        positions, row_ids, offsets, seq_lens, blocks = _batch(device, ids, n, n, table)
+        for d in (eager, graphed):
+            d.step(x0, positions, AdapterPlan(row_ids, 3), offsets, seq_lens, blocks)
+        x = torch.zeros((len(n), HIDDEN), dtype=torch.float16, device=device)
+        arrays = _batch(device, ids, n + 1, [1] * len(n), table)
+        state.append((x, arrays, AdapterPlan(arrays[1], 3)))
+
+    def step(decoder, i):
+        x, (positions, row_ids, offsets, seq_lens, blocks), plan = state[i]
+        plan.update(row_ids)
+        return decoder.step(x, positions, plan, offsets, seq_lens, blocks)
+
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step(graphed, i)
+        graphs.append((graph, held))
+    for turn in range(4):
+        for i in (1, 0):
+            lengths[i] += 1
+            x, (positions, row_ids, _, seq_lens, _), _ = state[i]
+            x.copy_(to_dev(rng.normal(0, 1 + turn, x.shape).astype(np.float16), device))
+            for mine, new in zip((positions, row_ids, seq_lens), (lengths[i] - 1, rng.integers(-1, 3, len(x)), lengths[i])):
+                mine.copy_(torch.tensor(new, dtype=torch.int32, device=device))
+            want = step(eager, i)
+            graphs[i][0].replay()
+            torch.cuda.synchronize()
+            for name, a, b in zip(("qkv", "q", "values", "y"), graphs[i][1], want):
+                assert torch.equal(a, b), (turn, i, name)
