@@ -46,9 +46,14 @@ def test_graphs_of_different_batches(hip, device, layers, dim, backward, rows):
     need = [(lib.gq_gemm_workspace_bytes if (dim == 0) != backward else lib.gq_linear_kn_workspace_bytes)(*s) for s in sizes]
     assert all(need) and len(set(need)) > 1
     xs = [torch.empty((m, IN), dtype=torch.float16, device=device) for m in rows]
-    graphs = [_captured(lambda x=x: call(x)) for x in xs]
-    owned = [id(ws) for _, ws in _gq_hip._captured_workspaces.values()]
-    assert owned and not set(owned) & {id(ws) for ws in _gq_hip._kn_workspaces.values()}
+    graphs, buffers = [], []
+    for x in xs:
+        before = {id(ws) for _, ws in _gq_hip._captured_workspaces.values()}
+        graphs.append(_captured(lambda: call(x)))
+        buffers += [b for b in _gq_hip._captured_workspaces.values() if id(b[1]) not in before]
+        assert len(buffers) == len(graphs)
+    assert len({number for number, _ in buffers}) == len({ws.data_ptr() for _, ws in buffers}) == len(rows)
+    assert not {ws.data_ptr() for _, ws in buffers} & {ws.data_ptr() for ws in _gq_hip._kn_workspaces.values()}
     streams = [torch.cuda.Stream(device=device) for _ in rows]
     for turn in range(4):
         for i, x in enumerate(xs):

@@ -303,7 +303,7 @@ def test_weights_dict_validates_dtype_and_shape():
         nt.missing
 
 
-def test_workspaces_of_captured_calls_are_their_capture_s(monkeypatch):
+def test_workspaces_of_captured_calls_belong_to_their_capture(monkeypatch):
     """A buffer of the arrival counters belongs to one stream's eager calls or to one stream of one capture: what a graph uses is
     zeroed by that graph, and no other graph or eager call writes there."""
     import contextlib
